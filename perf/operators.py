@@ -1,0 +1,383 @@
+"""Cases and plain forms of the attention operators that sit between the QKV and the output projection.
+
+  rotary   rotary positions of a [tokens, heads, head_dim] tensor, or the gradient of that
+  append   rotary positions of q and k, then k and v quantised to e4m3 into a paged cache, one scale per page and head
+  attend   attention of each sequence's newest tokens over that cache
+
+With `own` false `run` computes the operators from elementary torch operations; with `own` true it calls
+`tritonbench_b200.ops`.
+"""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+E4M3 = torch.float8_e4m3fn
+
+
+# ------------------------------------------------------------------ cases
+def _rotary(name, tokens, heads, dim, rot, interleaved, transpose, dtype, max_pos, factor=1.0):
+    return dict(name=name, op="rotary", tokens=tokens, heads=heads, dim=dim, rot=rot, interleaved=interleaved,
+                transpose=transpose, dtype=dtype, max_pos=max_pos, factor=factor)
+
+
+def _append(name, batch, new_max, ragged, ctx_max, heads, kv_heads, dim, rot, page, interleaved, dtype):
+    return dict(name=name, op="append", batch=batch, new_max=new_max, ragged=ragged, ctx_max=ctx_max, heads=heads,
+                kv_heads=kv_heads, dim=dim, rot=rot, page=page, interleaved=interleaved, dtype=dtype)
+
+
+def _attend(name, batch, new_max, ragged, ctx_min, ctx_max, heads, kv_heads, dim, page, dtype):
+    return dict(name=name, op="attend", batch=batch, new_max=new_max, ragged=ragged, ctx_min=ctx_min, ctx_max=ctx_max,
+                heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype)
+
+
+def listed():
+    return [
+        # one decode step of 64 requests, q and k heads of the fused projection in one view: launch latency
+        _rotary("rotary_step", 64, 72, 128, 128, False, False, "bf16", 8192),
+        # the prompt pass of a long batch: pure bandwidth
+        _rotary("rotary_prompt", 16384, 40, 128, 128, False, False, "bf16", 16384),
+        # the gradient in a training step with fp32 activations: neighbouring pairs, half of the head rotated,
+        # positions stretched fourfold; an odd number of tokens
+        _rotary("rotary_grad", 8191, 32, 128, 64, True, True, "fp32", 32768, 4.0),
+        # one new token of one request
+        _append("append_one", 1, 1, False, 4001, 64, 8, 128, 128, 64, False, "bf16"),
+        # one new token of each of 250 requests, a decode step under load
+        _append("append_step", 250, 1, False, 1024, 64, 8, 128, 128, 64, False, "bf16"),
+        # prompts of different lengths packed behind one another, some onto an earlier turn's context
+        _append("append_prompts", 13, 2500, True, 700, 64, 8, 128, 128, 64, False, "bf16"),
+        # a chunk of a long prompt; small pages and heads, neighbouring pairs, half of the head rotated
+        _append("append_chunk", 1, 5000, False, 3001, 32, 8, 64, 32, 16, True, "fp16"),
+        # one request in its first turn: latency
+        _attend("attend_short", 1, 1, False, 777, 777, 32, 8, 128, 64, "bf16"),
+        # one request over a long document: a long axis and few rows
+        _attend("attend_long", 1, 1, False, 131077, 131077, 64, 8, 128, 64, "bf16"),
+        # a decode step under load, contexts of every length
+        _attend("attend_batch", 64, 1, False, 1, 8192, 64, 8, 128, 64, "bf16"),
+        # drafted tokens checked at once: one to six new tokens a request
+        _attend("attend_drafts", 32, 6, True, 100, 6000, 64, 8, 128, 32, "bf16"),
+        # every query head with keys of its own, small heads and pages
+        _attend("attend_heads", 48, 1, False, 100, 3000, 32, 32, 64, 16, "fp16"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["rotary", "append", "attend", "attend"])
+    if op == "rotary":
+        dim = rng.choice([64, 128, 256])
+        heads = rng.choice([1, 8, 17, 32, 40, 72])
+        case = _rotary("", _log(rng, 1, min(16384, 40 * 16384 * 128 // (2 * heads * dim))), heads, dim,
+                       rng.choice([dim, dim // 2]), rng.random() < 0.5, rng.random() < 0.5,
+                       rng.choice(["bf16", "fp16", "fp32"]), rng.choice([16384, 32768]), rng.choice([1.0, 4.0, 8.0]))
+    elif op == "append":
+        dim = rng.choice([64, 128])
+        kv = rng.choice([1, 2, 8])
+        heads = kv * rng.choice([1, 4, 7, 8])
+        if rng.random() < 0.5:
+            batch, new, ragged = _log(rng, 1, 250), 1, False
+        else:
+            batch = _log(rng, 1, 32)
+            new, ragged = _log(rng, 2, min(16384, 16384 * 8192 // (heads * dim)) // batch), rng.random() < 0.7
+        case = _append("", batch, new, ragged, rng.randint(0, 1500), heads, kv, dim, rng.choice([dim, dim // 2]),
+                       rng.choice([16, 32, 64, 128]), rng.random() < 0.5, rng.choice(["bf16", "fp16"]))
+    else:
+        dim = rng.choice([64, 128, 128])
+        kv = rng.choice([1, 2, 4, 8])
+        group = rng.choice([1, 3, 4, 8, 8])
+        batch = _log(rng, 1, 128)
+        new = rng.choice([1, 1, 1, 2, 4, 6])
+        ctx = _log(rng, 1, min(131072, 240_000_000 // (batch * kv * dim)))
+        case = _attend("", batch, new, new > 1 and rng.random() < 0.6, rng.randint(1, ctx), ctx, kv * group, kv, dim,
+                       rng.choice([16, 32, 64, 128]), rng.choice(["bf16", "fp16"]))
+    del case["name"]
+    return case
+
+
+def _lengths(case):
+    """(tokens already there, new tokens) of every sequence: a part of the case, the same for every seed."""
+    gen = torch.Generator().manual_seed(20 + case["batch"])
+    b = case["batch"]
+    if case["op"] == "append":
+        old = torch.randint(0, case["ctx_max"] + 1, (b,), generator=gen)
+        if b == 1:
+            old = torch.tensor([case["ctx_max"]])
+    else:
+        old = torch.randint(case["ctx_min"], case["ctx_max"] + 1, (b,), generator=gen)
+        old[-1] = case["ctx_max"]
+    if case["ragged"]:
+        new = torch.randint(1, case["new_max"] + 1, (b,), generator=gen)
+    else:
+        new = torch.full((b,), case["new_max"])
+    if case["op"] == "attend":
+        old = (old - new).clamp(min=0)  # ctx counts the new tokens
+    return old, new
+
+
+# ------------------------------------------------------------------ inputs
+def _table(max_pos, rot, factor, device):
+    """[max_pos, rot]: cosines, then sines; positions divided by `factor` (contexts stretched linearly)."""
+    inv = 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+    angle = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] / factor * inv
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def _quantised_pages(pages, kv, page, dim, spread, gen, device):
+    """Pages as an earlier pass left them: e4m3 codes that fill the format's range, one power of two per page and head."""
+    codes = torch.empty((pages, kv, page, dim), dtype=E4M3, device=device)
+    scale = torch.empty((pages, kv), dtype=torch.float32, device=device)
+    step = max(1, (1 << 27) // (kv * page * dim))
+    for p in range(0, pages, step):
+        n = min(step, pages - p)
+        x = torch.randn((n, kv, page, dim), generator=gen, device=device) * spread
+        s = torch.exp2(torch.ceil(torch.log2(x.abs().amax(dim=(2, 3)) / 448)))
+        codes[p:p + n] = (x / s[:, :, None, None]).to(E4M3)
+        scale[p:p + n] = s
+    return codes, scale
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(int(seed))
+    host = torch.Generator().manual_seed(int(seed))
+    dtype = DTYPES[case["dtype"]]
+    if case["op"] == "rotary":
+        t, h, d = case["tokens"], case["heads"], case["dim"]
+        x = torch.randn((t, h, d), generator=gen, device=dev).to(dtype)
+        positions = torch.randint(0, case["max_pos"], (t,), generator=gen, device=dev)
+        return dict(case=case, x=x, positions=positions, table=_table(case["max_pos"], case["rot"], case["factor"], dev))
+    old, new = _lengths(case)
+    total = old + new
+    b, page, kv, d, h = case["batch"], case["page"], case["kv_heads"], case["dim"], case["heads"]
+    per_seq = (total + page - 1) // page
+    pages = int(per_seq.sum())
+    # the pages of a sequence lie anywhere in the cache
+    order = torch.randperm(pages, generator=host).to(torch.int32)
+    table = torch.zeros((b, int(per_seq.max())), dtype=torch.int32)
+    table[torch.arange(table.shape[1])[None, :] < per_seq[:, None]] = order
+    # keys of a real cache have a few strong channels
+    spread = 1 + 3 * (torch.rand(d, generator=gen, device=dev) < 0.05).float()
+    k, ks = _quantised_pages(pages, kv, page, d, spread, gen, dev)
+    v, vs = _quantised_pages(pages, kv, page, d, 1.0, gen, dev)
+    tokens = int(new.sum())
+    state = dict(case=case, block_table=table.to(dev), seq_lens=total.to(torch.int32).to(dev),
+                 k_cache=k, v_cache=v, k_scale=ks, v_scale=vs, old=old, new=new)
+    state["cu_seqlens"] = None
+    if case["new_max"] > 1:
+        state["cu_seqlens"] = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)]).to(torch.int32).to(dev)
+    if case["op"] == "append":
+        qkv = torch.randn((tokens, h + 2 * kv, d), generator=gen, device=dev)
+        qkv[:, h:h + kv] *= spread
+        qkv = qkv.to(dtype)  # what the QKV projection leaves: q, k and v are views of its rows
+        state.update(q=qkv[:, :h], k=qkv[:, h:h + kv], v=qkv[:, h + kv:],
+                     table=_table(int(total.max()), case["rot"], 1.0, dev))
+    else:
+        state["q"] = (torch.randn((tokens, h, d), generator=gen, device=dev) * 1.2).to(dtype)
+    return state
+
+
+# ------------------------------------------------------------------ plain forms
+def _rotate(x, cos, sin, rot, interleaved):
+    """x [tokens, heads, dim] in 32 bits, cos and sin [tokens, rot / 2]."""
+    c, s = cos[:, None, :], sin[:, None, :]
+    if interleaved:
+        a, b = x[..., 0:rot:2], x[..., 1:rot:2]
+        turned = torch.stack([a * c - b * s, b * c + a * s], dim=-1).flatten(-2)
+    else:
+        a, b = x[..., : rot // 2], x[..., rot // 2 : rot]
+        turned = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+    return torch.cat([turned, x[..., rot:]], dim=-1)
+
+
+def _plain_rotary(s):
+    case = s["case"]
+    half = case["rot"] // 2
+    rows = s["table"][s["positions"]]
+    sin = -rows[:, half:] if case["transpose"] else rows[:, half:]
+    return _rotate(s["x"].float(), rows[:, :half], sin, case["rot"], case["interleaved"]).to(s["x"].dtype)
+
+
+def _where(s):
+    """Sequence and position of every new token."""
+    lens = s["seq_lens"].long()
+    tokens = s["q"].shape[0]
+    t = torch.arange(tokens, device=lens.device)
+    cu = s["cu_seqlens"]
+    cu = torch.arange(lens.numel() + 1, device=lens.device) if cu is None else cu.long()
+    seq = torch.searchsorted(cu, t, right=True) - 1
+    first = lens - (cu[1:] - cu[:-1])
+    return seq, first[seq] + t - cu[seq], first
+
+
+def _store(x, codes, scale, seq, pos, first, block_table):
+    """Quantises x [tokens, kv, dim] into the pages; `codes` and `scale` are changed in place."""
+    size = codes.shape[2]
+    page, row = block_table[seq, pos // size].long(), pos % size
+    amax = torch.where(x.isfinite(), x.abs(), 0.0).amax(dim=-1)
+    need = torch.zeros_like(scale).index_reduce_(0, page, amax, "amax")
+    fraction, exponent = torch.frexp(need)  # the smallest power of two with need / scale <= 448 = 0.875 * 2^9
+    exponent = torch.where(fraction <= 0.875, exponent - 9, exponent - 8).clamp(min=-126)
+    need = torch.ldexp(torch.ones_like(need), exponent)
+    # the first page of a sequence may hold tokens already: they keep their codes, or move to the larger scale
+    held = first % size
+    at = block_table.gather(1, (first // size).clamp(max=block_table.shape[1] - 1)[:, None])[:, 0].long()
+    before = scale[at]
+    after = torch.where(held[:, None] > 0, torch.maximum(before, need[at]), need[at])
+    scale[page] = need[page]
+    goes_on = (held > 0)[:, None]
+    scale[at] = torch.where(goes_on, after, scale[at])
+    ratio = torch.where(goes_on, before / after, 1.0)[:, :, None, None]
+    there = codes[at]
+    keeps = (torch.arange(size, device=codes.device) < held[:, None])[:, None, :, None]
+    codes[at] = torch.where(keeps, (there.float() * ratio), there.float()).to(E4M3)
+    heads = torch.arange(codes.shape[1], device=codes.device)
+    codes.view(torch.uint8)[page[:, None], heads, row[:, None]] = (x * (1.0 / scale[page])[:, :, None]).to(E4M3).view(torch.uint8)
+
+
+def _plain_append(s):
+    case = s["case"]
+    half = case["rot"] // 2
+    seq, pos, first = _where(s)
+    rows = s["table"][pos]
+    cos, sin = rows[:, :half], rows[:, half:]
+    q = _rotate(s["q"].float(), cos, sin, case["rot"], case["interleaved"]).to(s["q"].dtype)
+    k = _rotate(s["k"].float(), cos, sin, case["rot"], case["interleaved"])
+    _store(k, s["k_cache"], s["k_scale"], seq, pos, first, s["block_table"])
+    _store(s["v"].float(), s["v_cache"], s["v_scale"], seq, pos, first, s["block_table"])
+    return dict(q=q, k=s["k_cache"], v=s["v_cache"], k_scale=s["k_scale"], v_scale=s["v_scale"])
+
+
+def _plain_attend(s):
+    """Keys, values and queries padded to the longest sequence: [batch, kv, rows, keys]."""
+    case = s["case"]
+    kv, d, group = case["kv_heads"], case["dim"], case["heads"] // case["kv_heads"]
+    table = s["block_table"].long()
+    b, size = table.shape[0], case["page"]
+    keys = table.shape[1] * size
+    new = case["new_max"]
+    seq, pos, first = _where(s)
+    slot = pos - first[seq]
+    q = torch.zeros((b, new, kv, group, d), dtype=torch.float32, device=table.device)
+    q[seq, slot] = s["q"].float().view(-1, kv, group, d)
+    q = q.permute(0, 2, 1, 3, 4).reshape(b, kv, new * group, d)
+    k = (s["k_cache"][table].float() * s["k_scale"][table][..., None, None]).transpose(1, 2).reshape(b, kv, keys, d)
+    score = (q @ k.transpose(-1, -2)) * d ** -0.5
+    del k
+    last = first[:, None] + torch.arange(new, device=table.device).repeat_interleave(group)  # [batch, rows]
+    hidden = torch.arange(keys, device=table.device) > last[:, :, None]
+    score = score.masked_fill_(hidden[:, None], float("-inf"))
+    score = (score - score.amax(dim=-1, keepdim=True)).exp_()
+    score = score / score.sum(dim=-1, keepdim=True)
+    v = (s["v_cache"][table].float() * s["v_scale"][table][..., None, None]).transpose(1, 2).reshape(b, kv, keys, d)
+    o = (score @ v).view(b, kv, new, group, d).permute(0, 2, 1, 3, 4).reshape(b, new, kv * group, d)
+    return o[seq, slot].to(s["q"].dtype)
+
+
+def run(state):
+    case = state["case"]
+    if not own:
+        return {"rotary": _plain_rotary, "append": _plain_append, "attend": _plain_attend}[case["op"]](state)
+    from tritonbench_b200 import ops
+
+    if case["op"] == "rotary":
+        return ops.rotary(state["x"], state["positions"], state["table"], interleaved=case["interleaved"],
+                          transpose=case["transpose"])
+    cache = ops.Fp8KvCache(state["k_cache"], state["v_cache"], state["k_scale"], state["v_scale"])
+    if case["op"] == "append":
+        q = ops.fp8_kv_append(state["q"], state["k"], state["v"], cache, state["block_table"], state["seq_lens"],
+                              cu_seqlens=state["cu_seqlens"], table=state["table"], interleaved=case["interleaved"])
+        return dict(q=q, k=cache.k, v=cache.v, k_scale=cache.k_scale, v_scale=cache.v_scale)
+    return ops.fp8_kv_attention(state["q"], cache, state["block_table"], state["seq_lens"],
+                                cu_seqlens=state["cu_seqlens"])
+
+
+def work(case):
+    size = 4 if case["dtype"] == "fp32" else 2
+    if case["op"] == "rotary":
+        t, n = case["tokens"], case["tokens"] * case["heads"] * case["dim"]
+        rotated = t * case["heads"] * case["rot"]
+        return {"bytes": 2 * n * size + t * (8 + 4 * case["rot"]), "flops": 3 * rotated}
+    old, new = _lengths(case)
+    t, kv, d, h, page = int(new.sum()), case["kv_heads"], case["dim"], case["heads"], case["page"]
+    if case["op"] == "append":
+        touched = int(((old + new - 1) // page - old // page + 1).sum())
+        return {"bytes": t * (2 * h * d * size + 2 * kv * d * (size + 1) + 4 * case["rot"]) + touched * (kv * 8 + 4) + 4 * len(old),
+                "flops": t * (3 * (h + kv) * case["rot"] + 4 * kv * d)}
+    total = old + new
+    held = int(total.sum())
+    pages = int(((total + page - 1) // page).sum())
+    seen = int((new * old + new * (new + 1) // 2).sum())
+    return {"bytes": 2 * held * kv * d + pages * (kv * 8 + 4) + 2 * t * h * d * size, "flops": 4 * seen * h * d}
+
+
+# ------------------------------------------------------------------ 64 bits, from the definitions
+def _turn64(x, angles, rot, interleaved, sign=1.0):
+    """Each pair of dimensions as a complex number, multiplied by (cos, sin) of its angle's table entry."""
+    z = x.double()
+    pairs = z[..., :rot].unflatten(-1, (rot // 2, 2)) if interleaved else z[..., :rot].unflatten(-1, (2, rot // 2)).transpose(-1, -2)
+    turned = torch.view_as_real(torch.view_as_complex(pairs.contiguous()) * torch.complex(angles[0], sign * angles[1])[:, None, :])
+    z[..., :rot] = (turned if interleaved else turned.transpose(-1, -2)).flatten(-2)
+    return z
+
+
+def _pages64(values, old_codes, old_scale, held):
+    """One page and head group: values [n, kv, dim] behind `held` rows of old codes [kv, page, dim]."""
+    finite = torch.where(values.isfinite(), values.abs(), 0.0)
+    need = torch.exp2(torch.ceil(torch.log2(finite.amax(dim=(0, 2)) / 448)).clamp(min=-126))
+    scale = torch.maximum(old_scale.double(), need) if held else need
+    codes = old_codes.double()
+    if held:
+        codes[:, :held] = (codes[:, :held] * (old_scale.double() / scale)[:, None, None]).to(E4M3).double()
+    codes[:, held:held + len(values)] = (values / scale[:, None]).to(E4M3).double().transpose(0, 1)
+    return codes, scale
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "rotary":
+        rows = s["table"].double()[s["positions"]]
+        half = case["rot"] // 2
+        x = s["x"].double()
+        return _turn64(x, (rows[:, :half], rows[:, half:]), case["rot"], case["interleaved"], -1.0 if case["transpose"] else 1.0)
+    old, new = s["old"].tolist(), s["new"].tolist()
+    page, kv, d, h = case["page"], case["kv_heads"], case["dim"], case["heads"]
+    pages = s["block_table"].cpu().tolist()
+    if case["op"] == "append":
+        half = case["rot"] // 2
+        at = torch.cat([torch.arange(o, o + n) for o, n in zip(old, new)]).to(s["q"].device)
+        rows = s["table"].double()[at]
+        angles = (rows[:, :half], rows[:, half:])
+        out = {"q": _turn64(s["q"].double(), angles, case["rot"], case["interleaved"])}
+        for name, x in (("k", _turn64(s["k"].double(), angles, case["rot"], case["interleaved"])), ("v", s["v"].double())):
+            codes, scale = s[name + "_cache"].double(), s[name + "_scale"].double()
+            base = 0
+            for b, (o, n) in enumerate(zip(old, new)):
+                t = 0
+                while t < n:
+                    held = (o + t) % page
+                    take = min(page - held, n - t)
+                    p = pages[b][(o + t) // page]
+                    codes[p], scale[p] = _pages64(x[base + t:base + t + take], codes[p], scale[p], held)
+                    t += take
+                base += n
+            out[name], out[name + "_scale"] = codes, scale
+        return out
+    outs, base = [], 0
+    for b, (o, n) in enumerate(zip(old, new)):
+        ids = torch.tensor(pages[b][: (o + n + page - 1) // page], device=s["q"].device)
+        # [keys, kv, dim]
+        k = (s["k_cache"][ids].double() * s["k_scale"][ids].double()[..., None, None]).transpose(1, 2).reshape(-1, kv, d)[: o + n]
+        v = (s["v_cache"][ids].double() * s["v_scale"][ids].double()[..., None, None]).transpose(1, 2).reshape(-1, kv, d)[: o + n]
+        q = s["q"][base:base + n].double().view(n, kv, h // kv, d)
+        score = torch.einsum("nkgd,jkd->nkgj", q, k) / math.sqrt(d)
+        for i in range(n):
+            score[i, :, :, o + i + 1:] = float("-inf")
+        weight = torch.softmax(score, dim=-1)
+        outs.append(torch.einsum("nkgj,jkd->nkgd", weight, v).reshape(n, h, d))
+        base += n
+    return torch.cat(outs)
