@@ -240,6 +240,77 @@ int b200fp8_fused_row_quantize(int producer, const void* x1_bf16, const void* x2
                                void* cuda_stream);
 
 /*
+ * Rotary positions: x [tokens, heads, dim] (element pitches per token and head, dim contiguous) -> y, out of place or
+ * in place (y == x).  For every pair (a, b) of the first rot elements of a head, (i, i + rot/2), or (2i, 2i + 1) with
+ * interleaved:   y_a = x_a c - x_b s,   y_b = x_b c + x_a s,   c and s from row positions[token] of `table`
+ * ([max_pos][rot] fp32: rot/2 cosines, then rot/2 sines).  Elements behind rot are copied.  transpose != 0: s -> -s,
+ * the gradient with regard to x.  fp32 arithmetic, one rounding.  A position outside the table gives NaN.
+ * Replaces: nothing in the reference's FP8 path (its projections stop at the QKV GEMM's output).
+ */
+int b200fp8_rotary(const void* x, int dtype, void* y, int64_t tokens, int64_t heads, int64_t dim, int64_t x_token,
+                   int64_t x_head, int64_t y_token, int64_t y_head, const void* positions, int positions_64,
+                   const float* table, int64_t max_pos, int64_t rot, int interleaved, int transpose, void* cuda_stream);
+
+/*
+ * A paged key/value cache in e4m3.  k, v: codes [num_pages][kv_heads][page_size][head_dim] with byte pitches per page,
+ * head and row (multiples of 16, head_dim contiguous); k_scale, v_scale: one fp32 scale per page and head with element
+ * pitches; value = code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The descriptor is read during
+ * the call; the memory it points to is the caller's.
+ */
+typedef struct b200fp8_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_pitch[3], v_pitch[3];             /* bytes: page, head, row */
+  int64_t k_scale_pitch[2], v_scale_pitch[2]; /* elements: page, head   */
+  int64_t num_pages, kv_heads, page_size, head_dim;
+} b200fp8_kv_cache;
+
+/*
+ * Which tokens belong to which sequence, for the two calls below (all arrays in device memory, never copied to the
+ * host): the rows of q, k, v are the newest tokens of `batch` sequences packed behind one another, those of sequence b
+ * from cu_seqlens[b] to cu_seqlens[b + 1] - one each when cu_seqlens is NULL.  seq_lens[b] is the length of the sequence
+ * with them, so its last row is at position seq_lens[b] - 1.  Position j lies in row j % page_size of page
+ * block_table[b * table_pitch + j / page_size].  Rows whose position would be negative (seq_lens[b] smaller than the
+ * number of rows; 0 for a padded entry of the batch), positions beyond the table's width and pages outside the cache
+ * are skipped: nothing is stored for them or read there.
+ */
+typedef struct b200fp8_kv_batch {
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int64_t table_pitch, table_width, batch, tokens;
+} b200fp8_kv_batch;
+
+/*
+ * Producer + quantiser into the cache: rotates q and k at their positions (as b200fp8_rotary, with rot a multiple of 16;
+ * table NULL: no rotation), writes q to q_out (q_out may be q; q NULL: no q), and stores k and v as e4m3.  The scale of
+ * a page and head is the smallest power of two (>= 2^-126) that takes the largest finite magnitude of its tokens to at
+ * most 448; when a page that already holds tokens needs a larger one, their codes are multiplied by old / new scale.
+ * Infinities and NaN are stored as NaN.  dtype of q, k, v: bf16 or fp16; element pitches per token and head, multiples
+ * of 8.  q_out rows of skipped tokens are zero; rows behind the last sequence are left as they were, or zeroed with
+ * fill_rest.  Two sequences must not append to the same page.
+ */
+int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t heads, int64_t q_token,
+                      int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t qo_token,
+                      int64_t qo_head, const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows, const float* table,
+                      int64_t max_pos, int64_t rot, int interleaved, int fill_rest, void* cuda_stream);
+
+/*
+ * Attention of the new tokens over the cache, the token itself and all before it: heads / kv_heads neighbouring query
+ * heads share a kv head,  o = sum_j softmax_j(softmax_scale * q . k_j) v_j.  q and out [tokens, heads, head_dim] bf16 or
+ * fp16, element pitches multiples of 8 (out: of 4); lse [tokens, heads] fp32 (natural logarithm of the softmax's
+ * denominator) or NULL.  A row without a token to see gives zeros, and lse = -infinity.  fill_rest as above for out; lse is
+ * -infinity behind the last sequence.
+ * The workspace needs no initialisation and may be reused as soon as the call has run; calls that overlap need one each.
+ */
+size_t b200fp8_kv_attention_workspace_bytes(const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows, int64_t heads);
+int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_t heads, int64_t q_token, int64_t q_head,
+                         int64_t o_token, int64_t o_head, const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows,
+                         float softmax_scale, int fill_rest, void* workspace, size_t workspace_bytes, void* cuda_stream);
+
+/*
  * Read the device status word of a workspace.  Call after the stream has been synchronised.
  * Returns B200FP8_OK or B200FP8_DEVICE_TIMEOUT; *device_status receives the raw word
  * (code << 24 | site).  Replaces: the reference's exit-on-error helper macros

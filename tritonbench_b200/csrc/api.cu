@@ -878,6 +878,211 @@ int b200fp8_fused_row_quantize(int producer, const void* x1, const void* x2, int
   return note_cuda(launch_fused_row_quantize(p, static_cast<cudaStream_t>(cuda_stream)));
 }
 
+int b200fp8_rotary(const void* x, int dtype, void* y, int64_t tokens, int64_t heads, int64_t dim, int64_t x_token,
+                   int64_t x_head, int64_t y_token, int64_t y_head, const void* positions, int positions_64,
+                   const float* table, int64_t max_pos, int64_t rot, int interleaved, int transpose, void* cuda_stream) {
+  if (tokens < 0 || heads <= 0 || dim <= 0 || rot < 2 || rot % 2 != 0 || rot > dim || max_pos <= 0) return B200FP8_BAD_ARG;
+  if (dtype < kQuantBf16 || dtype > kQuantFp32) return B200FP8_BAD_ARG;
+  if (tokens == 0) return B200FP8_OK;
+  if (x == nullptr || y == nullptr || positions == nullptr || table == nullptr) return B200FP8_BAD_ARG;
+  if (tokens > 0x7FFFFFFFll || heads > 0xFFFFFll || dim > 0xFFFFll || heads * dim > 0x7FFFFFFFll ||
+      tokens * heads > 0xFFFFFFFFFFll / dim) {
+    return B200FP8_TOO_LARGE;
+  }
+  const int64_t elem = dtype == kQuantFp32 ? 4 : 2;
+  RotaryParams p = {};
+  p.x = x;
+  p.y = y;
+  p.positions = positions;
+  p.table = table;
+  p.x_token = x_token;
+  p.x_head = x_head;
+  p.y_token = y_token;
+  p.y_head = y_head;
+  p.max_pos = max_pos;
+  p.tokens = static_cast<int>(tokens);
+  p.heads = static_cast<int>(heads);
+  p.dim = static_cast<int>(dim);
+  p.rot = static_cast<int>(rot);
+  p.dtype = dtype;
+  p.positions_64 = positions_64 ? 1 : 0;
+  p.interleaved = interleaved ? 1 : 0;
+  p.transpose = transpose ? 1 : 0;
+  p.copy_rest = x != y || x_token != y_token || x_head != y_head;
+  p.vector_ok = aligned16(x) && aligned16(y) && aligned16(table) && (x_token * elem) % 16 == 0 && (x_head * elem) % 16 == 0 &&
+                (y_token * elem) % 16 == 0 && (y_head * elem) % 16 == 0;
+  return note_cuda(launch_rotary(p, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+namespace {
+
+// what both calls on a paged cache ask of its descriptor and of the batch
+int check_kv(const b200fp8_kv_cache* c, const b200fp8_kv_batch* r, int64_t heads) {
+  if (c == nullptr || r == nullptr) return B200FP8_BAD_ARG;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  if (c->num_pages < 0 || c->kv_heads <= 0 || r->batch < 0 || r->tokens < 0 || r->table_width < 0) return B200FP8_BAD_ARG;
+  if (heads <= 0 || heads % c->kv_heads != 0) return B200FP8_BAD_ARG;
+  if (r->cu_seqlens == nullptr && r->tokens != r->batch) return B200FP8_BAD_ARG;
+  if (r->tokens == 0) return B200FP8_OK;
+  if (r->batch == 0 || r->seq_lens == nullptr) return B200FP8_BAD_ARG;
+  if (r->table_width > 0 && (r->block_table == nullptr || (r->batch > 1 && r->table_pitch < r->table_width))) return B200FP8_BAD_ARG;
+  if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr)) return B200FP8_BAD_ARG;
+  if (heads > 0xFFFFll || c->num_pages > 0x7FFFFFFFll || r->batch > 0xFFFFFFll || r->tokens > 0x3FFFFFFFll ||
+      r->tokens * heads > 0x3FFFFFFFll || r->table_width * c->page_size > 0x3FFFFFFFll) {
+    return B200FP8_TOO_LARGE;
+  }
+  if (!aligned16(c->k) || !aligned16(c->v)) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  for (int i = 0; i < 3; ++i) {
+    if (c->k_pitch[i] % 16 != 0 || c->v_pitch[i] % 16 != 0) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  }
+  return B200FP8_OK;
+}
+
+int log2_of(int64_t v) {
+  int s = 0;
+  while ((1ll << s) < v) ++s;
+  return s;
+}
+
+KvAttentionParams kv_attention_params(const b200fp8_kv_cache& c, const b200fp8_kv_batch& r, int64_t heads) {
+  KvAttentionParams p = {};
+  p.k_cache = static_cast<const uint8_t*>(c.k);
+  p.v_cache = static_cast<const uint8_t*>(c.v);
+  p.k_scale = c.k_scale;
+  p.v_scale = c.v_scale;
+  p.k_page = c.k_pitch[0];
+  p.k_head = c.k_pitch[1];
+  p.k_row = c.k_pitch[2];
+  p.v_page = c.v_pitch[0];
+  p.v_head = c.v_pitch[1];
+  p.v_row = c.v_pitch[2];
+  p.ks_page = c.k_scale_pitch[0];
+  p.ks_head = c.k_scale_pitch[1];
+  p.vs_page = c.v_scale_pitch[0];
+  p.vs_head = c.v_scale_pitch[1];
+  p.block_table = r.block_table;
+  p.bt_stride = r.table_pitch;
+  p.seq_lens = r.seq_lens;
+  p.cu_seqlens = r.cu_seqlens;
+  p.batch = static_cast<int>(r.batch);
+  p.tokens = static_cast<int>(r.tokens);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(c.kv_heads);
+  p.group = static_cast<int>(heads / c.kv_heads);
+  p.dim = static_cast<int>(c.head_dim);
+  p.page_size = static_cast<int>(c.page_size);
+  p.page_shift = log2_of(c.page_size);
+  p.num_pages = static_cast<int>(c.num_pages);
+  p.max_len = static_cast<int>(r.table_width * c.page_size);
+  return p;
+}
+
+}  // namespace
+
+int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t heads, int64_t q_token,
+                      int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t qo_token,
+                      int64_t qo_head, const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows, const float* table,
+                      int64_t max_pos, int64_t rot, int interleaved, int fill_rest, void* cuda_stream) {
+  const int st = check_kv(cache, rows, heads);
+  if (st != B200FP8_OK) return st;
+  if (dtype != kQuantBf16 && dtype != kQuantFp16) return B200FP8_BAD_ARG;
+  if (table != nullptr && (rot < 2 || rot % 2 != 0 || rot > cache->head_dim || max_pos <= 0)) return B200FP8_BAD_ARG;
+  if (rows->tokens == 0) return B200FP8_OK;
+  if (k == nullptr || v == nullptr || (q != nullptr && q_out == nullptr)) return B200FP8_BAD_ARG;
+  if (table != nullptr && (rot % 16 != 0 || !aligned16(table))) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  if (!aligned16(k) || !aligned16(v) || (k_token | k_head | v_token | v_head) % 8 != 0) return B200FP8_UNSUPPORTED_ALIGNMENT;
+  if (q != nullptr && (!aligned16(q) || !aligned16(q_out) || (q_token | q_head | qo_token | qo_head) % 8 != 0)) {
+    return B200FP8_UNSUPPORTED_ALIGNMENT;
+  }
+  KvAppendParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_out = q_out;
+  p.q_token = q_token;
+  p.q_head = q_head;
+  p.k_token = k_token;
+  p.k_head = k_head;
+  p.v_token = v_token;
+  p.v_head = v_head;
+  p.qo_token = qo_token;
+  p.qo_head = qo_head;
+  p.k_cache = static_cast<uint8_t*>(cache->k);
+  p.v_cache = static_cast<uint8_t*>(cache->v);
+  p.k_scale = cache->k_scale;
+  p.v_scale = cache->v_scale;
+  p.cache_page[0] = cache->k_pitch[0];
+  p.cache_head[0] = cache->k_pitch[1];
+  p.cache_row[0] = cache->k_pitch[2];
+  p.cache_page[1] = cache->v_pitch[0];
+  p.cache_head[1] = cache->v_pitch[1];
+  p.cache_row[1] = cache->v_pitch[2];
+  p.scale_page[0] = cache->k_scale_pitch[0];
+  p.scale_head[0] = cache->k_scale_pitch[1];
+  p.scale_page[1] = cache->v_scale_pitch[0];
+  p.scale_head[1] = cache->v_scale_pitch[1];
+  p.block_table = rows->block_table;
+  p.bt_stride = rows->table_pitch;
+  p.seq_lens = rows->seq_lens;
+  p.cu_seqlens = rows->cu_seqlens;
+  p.table = table;
+  p.max_pos = table != nullptr ? max_pos : 0;
+  p.batch = static_cast<int>(rows->batch);
+  p.tokens = static_cast<int>(rows->tokens);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(cache->kv_heads);
+  p.dim = static_cast<int>(cache->head_dim);
+  p.rot = table != nullptr ? static_cast<int>(rot) : 0;
+  p.page_size = static_cast<int>(cache->page_size);
+  p.page_shift = log2_of(cache->page_size);
+  p.table_width = static_cast<int>(rows->table_width);
+  p.num_pages = static_cast<int>(cache->num_pages);
+  p.dtype = dtype;
+  p.interleaved = interleaved ? 1 : 0;
+  p.fill_rest = fill_rest ? 1 : 0;
+  return note_cuda(launch_kv_append(p, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+size_t b200fp8_kv_attention_workspace_bytes(const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows, int64_t heads) {
+  if (check_kv(cache, rows, heads) != B200FP8_OK) return 0;
+  size_t bytes = 0;
+  if (note_cuda(launch_kv_attention(kv_attention_params(*cache, *rows, heads), &bytes, nullptr)) != B200FP8_OK) return 0;
+  return bytes;
+}
+
+int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_t heads, int64_t q_token, int64_t q_head,
+                         int64_t o_token, int64_t o_head, const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows,
+                         float softmax_scale, int fill_rest, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  const int st = check_kv(cache, rows, heads);
+  if (st != B200FP8_OK) return st;
+  if (dtype != kQuantBf16 && dtype != kQuantFp16) return B200FP8_BAD_ARG;
+  if (rows->tokens == 0) return B200FP8_OK;
+  if (q == nullptr || out == nullptr || workspace == nullptr) return B200FP8_BAD_ARG;
+  if (!aligned16(q) || (q_token | q_head) % 8 != 0 || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
+      (o_token | o_head) % 4 != 0 || !aligned16(workspace)) {
+    return B200FP8_UNSUPPORTED_ALIGNMENT;
+  }
+  KvAttentionParams p = kv_attention_params(*cache, *rows, heads);
+  size_t need = 0;
+  const int sized = note_cuda(launch_kv_attention(p, &need, nullptr));
+  if (sized != B200FP8_OK) return sized;
+  if (workspace_bytes < need) return B200FP8_WORKSPACE_TOO_SMALL;
+  p.q = q;
+  p.out = out;
+  p.lse = lse;
+  p.q_token = q_token;
+  p.q_head = q_head;
+  p.o_token = o_token;
+  p.o_head = o_head;
+  p.fp16 = dtype == kQuantFp16;
+  p.fill_rest = fill_rest ? 1 : 0;
+  p.softmax_scale = softmax_scale;
+  p.workspace = workspace;
+  p.workspace_bytes = workspace_bytes;
+  return note_cuda(launch_kv_attention(p, nullptr, static_cast<cudaStream_t>(cuda_stream)));
+}
+
 int b200fp8_selftest_wait_timeout(void* workspace, uint32_t limit_us, void* cuda_stream) {
   if (workspace == nullptr || limit_us == 0 || limit_us > 1000000u) return B200FP8_BAD_ARG;
   return note_cuda(launch_wait_timeout_selftest(static_cast<uint32_t*>(workspace),

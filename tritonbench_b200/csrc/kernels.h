@@ -290,4 +290,68 @@ struct FusedQuantParams {
 };
 cudaError_t launch_fused_row_quantize(const FusedQuantParams& p, cudaStream_t stream);
 
+// ------------------------ rotary positions (rotary.cu) ------------------------
+struct RotaryParams {
+  const void* x;  // [tokens, heads, dim], dim contiguous
+  void* y;        // same shape; may be x
+  const void* positions;  // [tokens] int32 or int64
+  const float* table;     // [max_pos][rot]: rot/2 cosines, rot/2 sines
+  long long x_token, x_head, y_token, y_head;  // elements
+  long long max_pos;
+  int tokens, heads, dim, rot;
+  int dtype;  // kQuant*
+  int positions_64, interleaved, transpose;
+  int copy_rest;  // the elements behind the rotated part are copied (out of place)
+  int vector_ok;  // x, y and table on 16-byte boundaries, pitches multiples of 16 bytes
+};
+cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t stream);
+
+// ------------------------ append to a paged e4m3 cache (kv_append.cu) ------------------------
+struct KvAppendParams {
+  const void *q, *k, *v;  // [tokens, heads or kv_heads, dim] bf16 or fp16; q may be null
+  void* q_out;            // q rotated; may be q
+  long long q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head;  // elements
+  uint8_t *k_cache, *v_cache;  // [num_pages][kv_heads][page_size][dim]
+  float *k_scale, *v_scale;    // [num_pages][kv_heads]
+  long long cache_page[2], cache_head[2], cache_row[2];  // bytes; k, v
+  long long scale_page[2], scale_head[2];                // elements
+  const int* block_table;  // [batch][table_width] page numbers
+  long long bt_stride;
+  const int* seq_lens;    // [batch] lengths, the new tokens included
+  const int* cu_seqlens;  // [batch + 1] first token of each sequence, or null: one token each
+  const float* table;     // as in RotaryParams; null with rot = 0
+  long long max_pos;
+  int batch, tokens, heads, kv_heads, dim, rot;
+  int page_size, page_shift, table_width, num_pages;
+  int dtype, interleaved;
+  int fill_rest;  // rows of q_out behind the last sequence are zeroed (else left as they are)
+};
+cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream);
+
+// ------------------------ attention over a paged e4m3 cache (kv_attention.cu) ------------------------
+struct KvAttentionParams {
+  const void* q;  // [tokens, heads, dim] bf16 or fp16
+  void* out;      // same
+  float* lse;     // [tokens, heads] or null
+  long long q_token, q_head, o_token, o_head;  // elements
+  const uint8_t *k_cache, *v_cache;            // as in KvAppendParams
+  const float *k_scale, *v_scale;
+  long long k_page, k_head, k_row, v_page, v_head, v_row;  // bytes
+  long long ks_page, ks_head, vs_page, vs_head;            // elements
+  const int* block_table;
+  long long bt_stride;
+  const int* seq_lens;
+  const int* cu_seqlens;
+  int batch, tokens, heads, kv_heads, group, dim;
+  int page_size, page_shift, num_pages;
+  int max_len;  // tokens that the block table has room for
+  int fp16;
+  int fill_rest;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes, parts_offset;
+};
+// bytes != null: only says how large a workspace this call needs
+cudaError_t launch_kv_attention(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream);
+
 }  // namespace b200fp8

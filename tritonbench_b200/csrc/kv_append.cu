@@ -1,0 +1,333 @@
+// Appending to a paged e4m3 cache, with the position rotation on the way: q and k are rotated at their sequence
+// positions, q is written back in its own type, k and v are quantised and stored into the pages of their sequence.
+//
+//   cache page p, kv head h:  codes [page_size][dim] e4m3, one fp32 scale;  value = code * scale[p][h]
+//   scale = the smallest power of two (>= 2^-126) with max |x| / scale <= 448 over the page's tokens of that head
+//   code  = e4m3(x * (1 / scale)), to nearest even
+//
+// The scale is a power of two because a page fills over many calls: when a later token needs a larger one, the codes
+// that are already there are multiplied by old / new, which is exact but for what falls below the format's smallest
+// subnormal.  It costs nothing in precision - e4m3 is a floating format, a power of two only moves its range by less
+// than one binade of its 15 - whereas an arbitrary scale would round the old codes anew each time it grows.
+// Infinities and NaN do not enter the scale (one bad value would take the page's other tokens with it) and are stored
+// as NaN.
+//
+// Bound by HBM for prompts (q in, q out, k and v in at 2 bytes, out at 1), by latency for single tokens.  One launch
+// does it all.  The first blocks own the pages: each group of threads has one (page, kv head, k or v), so that nothing
+// but that group reads or writes the page's scale: no atomics and the same result every time.  The remaining blocks
+// rotate q.  A group is a warp when a sequence brings about one token, else a block; it passes over its rows twice
+// (maximum, then codes), the second time out of L1.
+#include <cuda_fp8.h>
+
+#include "kernels.h"
+#include "rotary.cuh"
+
+namespace b200fp8 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kN = 8;  // elements of a 16-byte vector of bf16 or fp16; a slot is two of them
+
+// Sequence of a packed index: the largest b with key(b) <= at, by all lanes of a warp, 32 candidates a step.
+// key is not decreasing, key(0) <= at.
+template <typename Key>
+__device__ __forceinline__ int search_sequence(int batch, long long at, const Key& key) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = batch;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int b = lo + lane * step;
+    const bool below = lane * step < n && key(b) <= at;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1);
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.402823466e38f ? a : 0.0f;  // false for NaN
+}
+
+__device__ __forceinline__ float pow2_scale(float amax) {
+  // amax = m 2^(E - 127), m in [1, 2); 448 = 1.75 * 2^8
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23);  // biased exponent 1: 2^-126
+}
+
+__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float nan_for_inf(float v) { return fabsf(v) <= 3.402823466e38f ? v : __int_as_float(0x7fffffff); }
+
+__device__ __forceinline__ uint2 codes8(const float (&y)[kN], float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = codes2(nan_for_inf(y[4 * i]) * inv, nan_for_inf(y[4 * i + 1]) * inv) |
+           (codes2(nan_for_inf(y[4 * i + 2]) * inv, nan_for_inf(y[4 * i + 3]) * inv) << 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * i)), __NV_E4M3));
+    const float2 f = __half22float2(h);
+    out |= codes2(f.x * ratio, f.y * ratio) << (16 * i);
+  }
+  return out;
+}
+
+// Slot s of a head, at row x: vectors a and b at these elements.
+struct SlotAt {
+  int a, b;
+  bool turns;
+};
+template <bool kInterleaved>
+__device__ __forceinline__ SlotAt slot_at(int slot, int rot) {
+  if (slot < rot / (2 * kN)) {
+    if (kInterleaved) return {slot * 2 * kN, slot * 2 * kN + kN, true};
+    return {slot * kN, rot / 2 + slot * kN, true};
+  }
+  return {slot * 2 * kN, slot * 2 * kN + kN, false};  // rot is a multiple of a slot
+}
+
+template <bool kInterleaved>
+__device__ __forceinline__ void turn(const KvAppendParams& p, long long pos, int slot, float (&a)[kN], float (&b)[kN]) {
+  float c[kN], s[kN];
+  if (pos < p.max_pos) {
+    const float* row = p.table + pos * p.rot + slot * kN;
+    load_table<kN>(row, c);
+    load_table<kN>(row + p.rot / 2, s);
+  } else {  // the table ends before this position
+#pragma unroll
+    for (int i = 0; i < kN; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
+  }
+  rotate_slot<kN, kInterleaved>(a, b, c, s);
+}
+
+// One page, one kv head, k or v.  kGroup threads: a warp or the block.
+template <typename T, bool kInterleaved, int kGroup>
+__device__ __forceinline__ void append_page(const KvAppendParams& p, long long work) {
+  const int in_group = static_cast<int>(threadIdx.x) % kGroup;
+  const int which = static_cast<int>(work & 1);
+  const long long rest = work >> 1;
+  const int head = static_cast<int>(rest % p.kv_heads);
+  const long long slot_no = rest / p.kv_heads;
+  // slot_no -> sequence and page: sequence b owns the slots from cu[b] / page_size + 2 b on, at least as many as the
+  // pages that its tokens can touch
+  int b;
+  long long first_token, count, page_no;
+  if (p.cu_seqlens == nullptr) {
+    b = static_cast<int>(slot_no);
+    first_token = b;
+    count = 1;
+    page_no = 0;
+  } else {
+    const auto first_slot = [&](int i) { return static_cast<long long>(max(p.cu_seqlens[i], 0) >> p.page_shift) + 2ll * i; };
+    b = search_sequence(p.batch, slot_no, first_slot);
+    first_token = p.cu_seqlens[b];
+    count = p.cu_seqlens[b + 1] - first_token;
+    page_no = slot_no - first_slot(b);
+  }
+  const long long end = p.seq_lens[b];          // positions [begin, end) of the sequence are new
+  const long long begin = end - count;          // negative: more tokens than the sequence has; those are left out
+  if (count <= 0 || page_no < 0) return;
+  page_no += (begin > 0 ? begin : 0) >> p.page_shift;
+  if (page_no >= p.table_width) return;
+  const long long lo = page_no << p.page_shift;
+  const long long from = lo > begin ? lo : begin;
+  const long long to = lo + p.page_size < end ? lo + p.page_size : end;
+  if (from >= to) return;
+  const int page = p.block_table[b * p.bt_stride + page_no];
+  if (page < 0 || page >= p.num_pages) return;
+  const long long token0 = first_token + (from - begin);
+  const int rows = static_cast<int>(to - from);
+  if (token0 < 0 || token0 + rows > p.tokens) return;  // lengths that do not belong to this q, k, v
+  const int held = static_cast<int>(from - lo);
+
+  const T* x = which ? static_cast<const T*>(p.v) + token0 * p.v_token + head * p.v_head
+                     : static_cast<const T*>(p.k) + token0 * p.k_token + head * p.k_head;
+  const long long x_token = which ? p.v_token : p.k_token;
+  uint8_t* codes = (which ? p.v_cache : p.k_cache) + page * p.cache_page[which] + head * p.cache_head[which];
+  const long long code_row = p.cache_row[which];
+  float* scale_at = (which ? p.v_scale : p.k_scale) + page * p.scale_page[which] + head * p.scale_head[which];
+  const int rot = which ? 0 : p.rot;
+  const int slots = p.dim / (2 * kN);
+  const int items = rows * slots;
+  const float old_scale = held > 0 ? *scale_at : 0.0f;
+
+  const auto load = [&](int item, float (&a)[kN], float (&c)[kN], SlotAt& at) {
+    const int row = item / slots, slot = item - row * slots;
+    at = slot_at<kInterleaved>(slot, rot);
+    const T* r = x + row * x_token;
+    const uint4 ra = *reinterpret_cast<const uint4*>(r + at.a);
+    const uint4 rb = *reinterpret_cast<const uint4*>(r + at.b);
+    unpack16<T>(ra, a);
+    unpack16<T>(rb, c);
+    if (at.turns) turn<kInterleaved>(p, from + row, slot, a, c);
+    return row;
+  };
+
+  float amax = 0.0f;
+  for (int item = in_group; item < items; item += kGroup) {
+    float a[kN], c[kN];
+    SlotAt at;
+    load(item, a, c, at);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) amax = fmaxf(amax, fmaxf(finite_abs(a[i]), finite_abs(c[i])));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if constexpr (kGroup > 32) {
+    __shared__ float red[kThreads / 32];
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = red[0];
+#pragma unroll
+    for (int w = 1; w < kGroup / 32; ++w) amax = fmaxf(amax, red[w]);
+  } else {
+    __syncwarp();  // every lane has read the old scale before lane 0 writes the new one
+  }
+  const float need = pow2_scale(amax);
+  const float scale = fmaxf(old_scale, need);
+  const float inv = __fdiv_rn(1.0f, scale);
+  if (held > 0 && scale > old_scale) {  // the tokens that are already there move to the larger scale
+    const float ratio = __fdiv_rn(old_scale, scale);
+    const int vecs = p.dim / 16;
+    for (int i = in_group; i < held * vecs; i += kGroup) {
+      const int row = i / vecs;
+      uint4* at = reinterpret_cast<uint4*>(codes + row * code_row) + (i - row * vecs);
+      uint4 w = *at;
+      w.x = rescaled4(w.x, ratio);
+      w.y = rescaled4(w.y, ratio);
+      w.z = rescaled4(w.z, ratio);
+      w.w = rescaled4(w.w, ratio);
+      *at = w;
+    }
+  }
+  if (in_group == 0) *scale_at = scale;
+  for (int item = in_group; item < items; item += kGroup) {
+    float a[kN], c[kN];
+    SlotAt at;
+    const int row = load(item, a, c, at);
+    uint8_t* r = codes + (held + row) * code_row;
+    *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv);
+    *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv);
+  }
+}
+
+// kItems slots of q a thread; the positions of the block's tokens are looked up once, in shared memory
+constexpr int kItems = 2;
+constexpr int kMaxTokens = kThreads * kItems / 4 + 1;  // a head has at least four slots
+
+template <typename T, bool kInterleaved>
+__device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long block) {
+  __shared__ long long positions[kMaxTokens];
+  const int slots = p.dim / (2 * kN);
+  const unsigned per_token = static_cast<unsigned>(p.heads) * static_cast<unsigned>(slots);
+  const long long first = block * (kThreads * kItems);
+  const long long items = static_cast<long long>(p.tokens) * per_token;
+  const long long token0 = first / per_token;
+  const long long in_token0 = first - token0 * per_token;
+  long long token1 = (first + kThreads * kItems - 1) / per_token;
+  if (token1 >= p.tokens) token1 = p.tokens - 1;
+  uint4 ra[kItems], rb[kItems];
+  int local[kItems], head[kItems], slot[kItems];
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {  // on their way while the positions are looked up
+    const unsigned at = static_cast<unsigned>(in_token0) + threadIdx.x + j * kThreads;
+    local[j] = static_cast<int>(at / per_token);
+    const unsigned in_token = at - local[j] * per_token;
+    head[j] = static_cast<int>(in_token / static_cast<unsigned>(slots));
+    slot[j] = static_cast<int>(in_token - head[j] * static_cast<unsigned>(slots));
+    if (first + threadIdx.x + j * kThreads < items) {
+      const T* x = static_cast<const T*>(p.q) + (token0 + local[j]) * p.q_token + head[j] * p.q_head;
+      const SlotAt e = slot_at<kInterleaved>(slot[j], p.rot);
+      ra[j] = *reinterpret_cast<const uint4*>(x + e.a);
+      rb[j] = *reinterpret_cast<const uint4*>(x + e.b);
+    }
+  }
+  const int tokens = static_cast<int>(token1 - token0) + 1;
+  // all warps look up the block's tokens, one token a warp at a time
+  for (int i = threadIdx.x >> 5; i < tokens; i += kThreads / 32) {
+    const long long t = token0 + i;
+    long long pos;
+    if (p.cu_seqlens == nullptr) {
+      pos = p.seq_lens[t] - 1ll;
+    } else if (t >= p.cu_seqlens[p.batch]) {
+      pos = -2;  // behind the last sequence
+    } else {
+      const int b = search_sequence(p.batch, t, [&](int s) { return static_cast<long long>(p.cu_seqlens[s]); });
+      pos = p.seq_lens[b] - static_cast<long long>(p.cu_seqlens[b + 1]) + t;
+      if (pos < 0) pos = -1;
+    }
+    if ((threadIdx.x & 31) == 0) positions[i] = pos;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    if (first + threadIdx.x + j * kThreads >= items) continue;
+    const long long pos = positions[local[j]];
+    if (pos == -2 && !p.fill_rest) continue;
+    T* y = static_cast<T*>(p.q_out) + (token0 + local[j]) * p.qo_token + head[j] * p.qo_head;
+    const SlotAt e = slot_at<kInterleaved>(slot[j], p.rot);
+    float a[kN], b[kN];
+    unpack16<T>(ra[j], a);
+    unpack16<T>(rb[j], b);
+    if (pos < 0) {  // not a token of any sequence
+#pragma unroll
+      for (int i = 0; i < kN; ++i) a[i] = b[i] = 0.0f;
+    } else if (e.turns) {
+      turn<kInterleaved>(p, pos, slot[j], a, b);
+    }
+    *reinterpret_cast<uint4*>(y + e.a) = pack16<T>(a);
+    *reinterpret_cast<uint4*>(y + e.b) = pack16<T>(b);
+  }
+}
+
+template <typename T, bool kInterleaved, int kGroup>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks) {
+  if (blockIdx.x < page_blocks) {
+    constexpr int kPerBlock = kThreads / kGroup;
+    const long long work = static_cast<long long>(blockIdx.x) * kPerBlock + threadIdx.x / kGroup;
+    if (work < works) append_page<T, kInterleaved, kGroup>(p, work);
+  } else {
+    rotate_q<T, kInterleaved>(p, static_cast<long long>(blockIdx.x - page_blocks));
+  }
+}
+
+template <typename T, bool kInterleaved, int kGroup>
+cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
+  const long long page_slots = p.cu_seqlens == nullptr ? p.batch : (p.tokens >> p.page_shift) + 2ll * p.batch;
+  const long long works = page_slots * p.kv_heads * 2;
+  const long long page_blocks = (works + kThreads / kGroup - 1) / (kThreads / kGroup);
+  const long long items = p.q == nullptr ? 0 : static_cast<long long>(p.tokens) * p.heads * (p.dim / (2 * kN));
+  const long long q_blocks = (items + kThreads * kItems - 1) / (kThreads * kItems);
+  if (page_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (page_blocks + q_blocks == 0) return cudaSuccess;
+  kv_append_kernel<T, kInterleaved, kGroup><<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(
+      p, works, static_cast<unsigned>(page_blocks));
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_any(const KvAppendParams& p, cudaStream_t stream) {
+  // about one token a sequence: a block for every page would leave nearly all of its threads idle
+  const bool warps = p.cu_seqlens == nullptr || p.tokens <= 2ll * p.batch;
+  if (p.interleaved) return warps ? launch_t<T, true, 32>(p, stream) : launch_t<T, true, kThreads>(p, stream);
+  return warps ? launch_t<T, false, 32>(p, stream) : launch_t<T, false, kThreads>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream) {
+  return p.dtype == kQuantBf16 ? launch_any<__nv_bfloat16>(p, stream) : launch_any<__half>(p, stream);
+}
+
+}  // namespace b200fp8

@@ -5,6 +5,7 @@ There is no CPU or PyTorch fallback behind these calls.
 """
 import ctypes
 import os
+import struct
 from typing import Optional
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -49,6 +50,10 @@ VARIANTS = {
     "gemv": VARIANT_GEMV,
 }
 WORKSPACE_HEADER_BYTES = 256
+# b200fp8_kv_cache: k, v, k_scale, v_scale; k, v pitches (page, head, row), scale pitches; pages, heads, page size, dim
+KV_CACHE = struct.Struct("4P14q")
+# b200fp8_kv_batch: block_table, seq_lens, cu_seqlens; table pitch and width, batch, tokens
+KV_BATCH = struct.Struct("3P4q")
 IPC_HANDLE_BYTES = 64
 
 # every symbol include/b200fp8.h declares
@@ -79,6 +84,10 @@ EXPORTED_SYMBOLS = (
     "b200fp8_gemm_rowwise_grouped",
     "b200fp8_selftest_wait_timeout",
     "b200fp8_gemm_blockwise",
+    "b200fp8_rotary",
+    "b200fp8_kv_append",
+    "b200fp8_kv_attention_workspace_bytes",
+    "b200fp8_kv_attention",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -164,6 +173,19 @@ def load() -> ctypes.CDLL:
                                            c_int64, c_void_p]
     lib.b200fp8_row_quantize.restype = ctypes.c_int
     lib.b200fp8_row_quantize.argtypes = [c_void_p, ctypes.c_int, ctypes.c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]
+    c_int = ctypes.c_int
+    lib.b200fp8_rotary.restype = c_int
+    lib.b200fp8_rotary.argtypes = ([c_void_p, c_int, c_void_p] + [c_int64] * 7 + [c_void_p, c_int, c_void_p, c_int64, c_int64]
+                                   + [c_int, c_int, c_void_p])
+    # the cache and batch descriptors are packed by KV_CACHE and KV_BATCH below
+    lib.b200fp8_kv_append.restype = c_int
+    lib.b200fp8_kv_append.argtypes = ([c_void_p] * 4 + [c_int] + [c_int64] * 9 + [c_void_p] * 3 + [c_int64, c_int64]
+                                      + [c_int, c_int, c_void_p])
+    lib.b200fp8_kv_attention_workspace_bytes.restype = c_size_t
+    lib.b200fp8_kv_attention_workspace_bytes.argtypes = [c_void_p, c_void_p, c_int64]
+    lib.b200fp8_kv_attention.restype = c_int
+    lib.b200fp8_kv_attention.argtypes = ([c_void_p] * 3 + [c_int] + [c_int64] * 5 + [c_void_p] * 2
+                                         + [ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p])
     if lib.b200fp8_abi_version() != 1:
         raise RuntimeError("libb200fp8.so has an ABI version this binding does not know")
     _lib = lib

@@ -6,6 +6,7 @@ Mirrors the call the reference backends make,
 (tritonbench/operators/fp8_gemm_rowwise/operator.py:187-217): same argument order and meaning,
 a fresh bf16 [M, N] tensor as the result.
 """
+import contextlib
 from typing import Callable, Dict, Optional, Sequence, Tuple
 
 import torch
@@ -329,6 +330,268 @@ def fp8_gemm(a: torch.Tensor, b: torch.Tensor, scale_a=None, scale_b=None, out_d
         return s.reshape(-1).expand(count).contiguous() if s.numel() == 1 else s.reshape(count).contiguous()
 
     return fp8_gemm_rowwise(a, b.t(), vec(scale_a, m), vec(scale_b, n), out_dtype=out_dtype, **kw)
+
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on_device_of(t: torch.Tensor):
+    """Context in which t's device is the current one (a launch on a stream of another device is an error)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, table, interleaved, transpose):
+        ctx.save_for_backward(positions, table)
+        ctx.form = (interleaved, transpose)
+        return _rotary(x, positions, table, interleaved, transpose, None)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, table = ctx.saved_tensors
+        interleaved, transpose = ctx.form
+        if grad.stride(2) != 1:
+            grad = grad.contiguous()
+        return rotary(grad, positions, table, interleaved, not transpose), None, None, None, None
+
+
+def _rotary(x, positions, table, interleaved, transpose, out):
+    tokens, heads, dim = x.shape
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    if tokens == 0 or heads == 0:
+        return out
+    sx, sy = x.stride(), out.stride()
+    with _on_device_of(x):
+        status = _lib.load().b200fp8_rotary(
+            x.data_ptr(), _DTYPES[x.dtype], out.data_ptr(), tokens, heads, dim, sx[0], sx[1], sy[0], sy[1],
+            positions.data_ptr(), positions.dtype == torch.int64, table.data_ptr(), table.shape[0], table.shape[1],
+            interleaved, transpose, _stream(x.device),
+        )
+    _lib.check(status, f"b200fp8_rotary({tokens}x{heads}x{dim}, {x.dtype})")
+    return out
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interleaved: bool = False,
+           transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions of x [tokens, heads, dim] (bf16, fp16 or fp32; any token and head stride, so a view of a fused
+    projection's output will do): y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for the pairs (i, i + rot/2) - or
+    (2i, 2i + 1) if interleaved - of the first rot elements of a head, the others copied.  positions [tokens] int32 or
+    int64; table float32 [max_positions, rot] from `rotary.rotary_table`; a position outside it gives NaN.
+    fp32 arithmetic, one rounding.  out may be x.  transpose=True is the gradient with regard to x; a call on an x that
+    requires one is differentiable."""
+    for t, name in ((x, "x"), (positions, "positions"), (table, "table")):
+        _require_cuda(t, name)
+        if t.device != x.device:
+            raise ValueError(f"{name} must be on x's device")
+    if x.dim() != 3 or x.stride(2) != 1:
+        raise ValueError("x must be [tokens, heads, dim] with dim contiguous")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int32 or int64 vector")
+    if positions.numel() != x.shape[0]:
+        raise ValueError("positions must have one entry per token")
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+        raise ValueError("table must be a contiguous float32 [max_positions, rot]")
+    if not 2 <= table.shape[1] <= x.shape[2] or table.shape[1] % 2:
+        raise ValueError("the table's width must be even and at most dim")
+    interleaved, transpose = bool(interleaved), bool(transpose)
+    if torch.is_grad_enabled() and x.requires_grad:
+        if out is not None:
+            raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
+        return _Rotary.apply(x, positions, table, interleaved, transpose)
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+            raise ValueError("out must have x's shape, dtype and device, dim contiguous")
+    return _rotary(x, positions, table, interleaved, transpose, out)
+
+
+class Fp8KvCache:
+    """A paged key/value cache in e4m3: k and v [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn (any page, head
+    and row strides that are multiples of 16; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads] float32;
+    a value is code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object describes the four tensors
+    and keeps them alive; make one with `empty`, or around tensors of your own."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "descriptor")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        for t, name in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            _require_cuda(t, name)
+            if t.device != k.device:
+                raise ValueError("the cache's tensors must be on one device")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+            raise ValueError("k and v must be float8_e4m3fn [num_pages, kv_heads, page_size, head_dim]")
+        pages, heads, size, dim = k.shape
+        if heads < 1:
+            raise ValueError("a cache needs at least one kv head")
+        for s in (k_scale, v_scale):
+            if s.dtype != torch.float32 or tuple(s.shape) != (pages, heads):
+                raise ValueError("k_scale and v_scale must be float32 [num_pages, kv_heads]")
+        if size not in (16, 32, 64, 128) or dim not in (64, 128, 256):
+            raise NotImplementedError(f"page_size {size}, head_dim {dim}: page_size must be 16, 32, 64 or 128, head_dim 64, 128 or 256")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("head_dim must be contiguous in k and v")
+        for t in (k, v):
+            if t.data_ptr() % 16 or any(st % 16 for st in t.stride()[:3]):
+                raise NotImplementedError("rows of k and v must start on 16-byte boundaries")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
+        self.descriptor = _lib.KV_CACHE.pack(
+            k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+            *k_scale.stride(), *v_scale.stride(), pages, heads, size, dim)
+
+    @classmethod
+    def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "Fp8KvCache":
+        """A cache without tokens (codes and scales zero)."""
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+
+def _check_rows(x: torch.Tensor, name: str, cache: Fp8KvCache) -> None:
+    if x.device != cache.k.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    if x.dim() != 3 or x.shape[2] != cache.head_dim or x.stride(2) != 1:
+        raise ValueError(f"{name} must be [tokens, heads, {cache.head_dim}] with head_dim contiguous")
+    if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
+        raise ValueError(f"{name} must be bfloat16 or float16")
+
+
+def _pack_batch(tokens: int, cache: Fp8KvCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                cu_seqlens: Optional[torch.Tensor]) -> bytes:
+    device = cache.k.device
+    if block_table.device != device or seq_lens.device != device:
+        raise ValueError("block_table and seq_lens must be on the cache's device")
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous int32 vector")
+    batch = seq_lens.shape[0]
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError("block_table must be int32 [batch, pages]")
+    width = block_table.shape[1]
+    if width > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table must have its pages contiguous")
+    if cu_seqlens is None:
+        if tokens != batch:
+            raise ValueError(f"{tokens} tokens for {batch} sequences: pass cu_seqlens unless every sequence has one")
+        cu = 0
+    else:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] != batch + 1:
+            raise ValueError("cu_seqlens must be a contiguous int32 vector with batch + 1 entries")
+        if cu_seqlens.device != device:
+            raise ValueError("cu_seqlens must be on the cache's device")
+        cu = cu_seqlens.data_ptr()
+    return _lib.KV_BATCH.pack(block_table.data_ptr(), seq_lens.data_ptr(), cu, max(block_table.stride(0), width), width, batch, tokens)
+
+
+def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                  interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Rotary positions of q and k, then k and v quantised to e4m3 into the pages of their sequences, in one launch.
+    Returns the rotated q (None if q is None).
+
+    q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim], bf16 or fp16, any token and head strides that are
+    multiples of 8: views of the QKV projection's output will do.  The rows are the newest tokens of the batch's sequences
+    behind one another, cu_seqlens [batch + 1] their bounds (None: one each).  seq_lens [batch] counts them, so the last
+    row of sequence b has position seq_lens[b] - 1, and position j lies in page block_table[b, j // page_size].  All
+    three are int32 on the device and never copied to the host.  table: `rotary.rotary_table` (its width a multiple of
+    16), None for no rotation.
+
+    One scale per page and kv head: the smallest power of two that takes the page's largest finite magnitude to at most
+    448.  A page that already holds tokens keeps its scale, or is moved to a larger one.  Infinities and NaN are stored as
+    NaN.  Rows whose position would be negative (seq_lens[b] = 0: a padded entry), positions behind the block table and
+    pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q) keeps its rows
+    behind cu_seqlens[-1]; in a fresh result they are zero.  Two sequences must not append to the same page."""
+    if not isinstance(cache, Fp8KvCache):
+        raise ValueError("cache must be an Fp8KvCache")
+    _check_rows(k, "k", cache)
+    _check_rows(v, "v", cache)
+    if k.shape != v.shape or k.shape[1] != cache.kv_heads or k.dtype != v.dtype:
+        raise ValueError(f"k and v must be [tokens, {cache.kv_heads}, {cache.head_dim}] of one dtype")
+    tokens, heads = k.shape[0], cache.kv_heads
+    sk, sv = k.stride(), v.stride()
+    sq = so = (0, 0)
+    fill = 0
+    q_ptr = qo_ptr = None
+    if q is not None:
+        _check_rows(q, "q", cache)
+        heads = q.shape[1]
+        if q.shape[0] != tokens or q.dtype != k.dtype or heads < 1 or heads % cache.kv_heads:
+            raise ValueError("q must have k's tokens and dtype, and a multiple of its heads")
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+            fill = 1
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or q_out.stride(2) != 1:
+            raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
+        sq, so, q_ptr, qo_ptr = q.stride(), q_out.stride(), q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    max_pos = rot = 0
+    table_ptr = None
+    if table is not None:
+        if table.device != k.device or table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+            raise ValueError("table must be a contiguous float32 [max_positions, rot] on the cache's device")
+        max_pos, rot = table.shape
+        if not 2 <= rot <= cache.head_dim or rot % 2:
+            raise ValueError("the table's width must be even and at most head_dim")
+        table_ptr = table.data_ptr()
+    rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
+    with _on_device_of(k):
+        status = _lib.load().b200fp8_kv_append(
+            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, _DTYPES[k.dtype], heads, sq[0], sq[1], sk[0], sk[1], sv[0], sv[1],
+            so[0], so[1], cache.descriptor, rows, table_ptr, max_pos, rot, bool(interleaved), fill, _stream(k.device))
+    if status:
+        _lib.check(status, f"b200fp8_kv_append(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={cache.head_dim})")
+    return q_out
+
+
+def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                     cu_seqlens: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of the newest tokens of every sequence over the cache, each token over itself and all before it
+    (a decode step, drafted tokens, a chunk of a prompt).  q [tokens, heads, head_dim] bf16 or fp16; heads / kv_heads
+    neighbouring query heads share a kv head; block_table, seq_lens, cu_seqlens as for fp8_kv_append, which has stored the
+    tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
+    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads].
+
+    Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
+    (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows behind
+    cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for up to a few dozen new
+    tokens a sequence: the cache is read once per 16 query rows, with the work split over the context.  The result does
+    not depend on timing.  The workspace is allocated per call, so captured graphs and streams never share one."""
+    if not isinstance(cache, Fp8KvCache):
+        raise ValueError("cache must be an Fp8KvCache")
+    _check_rows(q, "q", cache)
+    tokens, heads, dim = q.shape
+    if heads < 1 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {cache.kv_heads} kv heads")
+    fill = 0
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        fill = 1
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+        raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
+    if tokens:
+        lib = _lib.load()
+        sq, so = q.stride(), out.stride()
+        with _on_device_of(q):
+            nbytes = lib.b200fp8_kv_attention_workspace_bytes(cache.descriptor, rows, heads)
+            ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+            status = lib.b200fp8_kv_attention(
+                q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), _DTYPES[q.dtype], heads, sq[0], sq[1],
+                so[0], so[1], cache.descriptor, rows, dim ** -0.5 if softmax_scale is None else softmax_scale, fill,
+                ws.data_ptr(), ws.numel(), _stream(q.device))
+        if status:
+            _lib.check(status, f"b200fp8_kv_attention(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={dim})")
+    return (out, lse) if return_lse else out
 
 
 def make_gemm_fn(xq, wq, x_scale, w_scale, bias=None, variant: str = "auto", reuse_out: bool = False,
