@@ -4,10 +4,12 @@ Usage: python -m tritonbench_b200.csrc.build [--force] [--verbose]
 The library is written next to this file; it links the CUDA runtime statically and needs
 nothing but the NVIDIA driver at run time.
 """
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_skinny.cu", "gemm_simt.cu", "quantize.cu", "fused_quantize.cu", "gemm_splitk.cu", "gemm_blockwise.cu", "gemm_gemv.cu",
@@ -40,21 +42,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
     out = lib_path()
     if not force and not needs_build():
         return out
-    cmd = [
-        _nvcc(),
+    flags = [
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-lineinfo", "-O3", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC",
+        "-Xcompiler", "-fPIC",
         "-cudart", "static",
     ]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", out] + [os.path.join(HERE, s) for s in SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if verbose:
-        print(res.stdout + res.stderr)
+        flags += ["-Xptxas", "-v"]
+
+    def run(args):
+        res = subprocess.run([_nvcc()] + flags + args, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            print(res.stdout + res.stderr)
+
+    with tempfile.TemporaryDirectory() as tmp, concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = [os.path.join(tmp, s.replace(".cu", ".o")) for s in SOURCES]
+        list(pool.map(lambda so: run(["-c", os.path.join(HERE, so[0]), "-o", so[1]]), zip(SOURCES, objects)))
+        run(["-shared", "-o", out] + objects)
     return out
 
 

@@ -15,10 +15,8 @@
 //     output stay in fp32.
 //   * The order of the contraction is free, so a thread's operand elements are 16 neighbouring bytes of a token:
 //     whole 16-byte vectors are loaded, and the pairing of two tokens' V bytes costs one byte permute per 4 bytes.
-//     Nothing is transposed through shared memory, and a thread reads only vectors that it copied itself (cp.async,
-//     [stage][vector][lane]): the ring needs no barrier and has no bank conflict.
-//   * v_scale differs by page and is applied in fp32 when a chunk's product is added to O, together with the
-//     rescaling that a new maximum asks for.
+//     A warp copies (cp.async, whole rows) and reads its own chunks, so the ring needs no barrier beyond the warp.
+//   * v_scale differs by page: O is kept in units of the V scale that was added last, so products accumulate in place.
 // Work is split over the context: all (sequence, kv head, row tile, unit of 4 chunks) units of the batch are one list,
 // cut into equal runs for a grid that fills the GPU once; lengths are read on the device.  A run that ends inside a
 // tile leaves its unnormalised sums in the workspace (at most two parts a CTA) and the second kernel joins them, in a
@@ -37,18 +35,24 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kMaxFloat = 3.402823466e38f;
+constexpr float kMinusInf = -__builtin_inff();
 constexpr uint32_t kNoPage = 0xffffffffu;  // in place of a chunk's k_scale: its page is not in the cache
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take) {  // zeros where not taken
+template <int kBytes, bool kAlways = true>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take = true) {  // zeros where not taken
   const int n = take ? kBytes : 0;
-  if constexpr (kBytes == 16) {
+  if constexpr (kBytes == 16 && kAlways) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  } else if constexpr (kBytes == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  } else if constexpr (kAlways) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
   } else {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(n) : "memory");
   }
@@ -57,17 +61,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int kPending>
 __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
 }
 
 // four e4m3 bytes -> bytes (0, 1) and bytes (2, 3) as fp16 pairs, exact
@@ -172,21 +165,44 @@ struct Cursor {
   }
 };
 
-template <int kD, int kNT, int kChunk, int kStages>
+// A warp takes kChunk tokens a step, 8 KB of codes, in parts of kSub tokens that lie in one page each.
+template <int kD, int kNT, int kSub>
 struct Shape {
+  static constexpr int kStages = 2;
   static constexpr int kRows = 8 * kNT;
+  static constexpr int kChunk = 4096 / kD;
+  static constexpr int kSubs = kChunk / kSub;
   static constexpr int kUnit = kWarps * kChunk;
   static constexpr int kMT = kChunk / 16;
-  static constexpr int kKVecs = (kChunk / 8) * (kD / 64);  // 16-byte vectors of K a lane has of a chunk
-  static constexpr int kVBytes = kD >= 128 ? 16 : 8;       // a lane's vector of V
-  static constexpr int kVH = kD >= 128 ? kD / 128 : 1;     // vectors of V per token
-  static constexpr int kVVecs = (kChunk / 4) * kVH;
-  static constexpr int kStageBytes = 32 * (16 * kKVecs + kVBytes * kVVecs + 8);
+  static constexpr int kTileBytes = kChunk * kD;               // codes of K or of V of a chunk
+  static constexpr int kStageBytes = 2 * kTileBytes + 32;      // and the scales of its parts
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kPitch = kD + 4;  // floats of a row of the warps' partial O
-  static constexpr int kMergeBytes = kWarps * kRows * kPitch * 4 + kWarps * kRows * 2 * 4;
-  static constexpr int kSmemBytes = kRingBytes + kMergeBytes;
+  static constexpr int kVW = kD >= 128 ? 4 : 2;                // words of V a lane has of a token and 128 elements
+  static constexpr int kVH = kD >= 128 ? kD / 128 : 1;
+  static constexpr int kOT = 2 * kVW;                          // 16-row tiles of O^T per vector of V
+  static constexpr int kQBytes = kRows * kD * 2;               // queries in fp16
+  // the warps of a block join their O, 8 KB of rows at a time, where the chunk lay that each multiplied last
+  static constexpr int kJoinNT = kNT < 256 / kD ? kNT : 256 / kD;
+  static constexpr int kSmemBytes = kRingBytes + kQBytes;
+  static_assert(kJoinNT * 8 * kD * 4 <= 2 * kTileBytes && kSubs <= 4 && kSub % 16 == 0 && kNT % kJoinNT == 0, "");
 };
+
+// Where row and 16-byte vector c of a chunk's K or V lie in shared memory, in bytes.  A copy instruction writes whole
+// rows (full lines in global memory: 6.8 TB/s of random 4 KB pieces, where a lane that fetched the vectors it reads
+// itself, 64 bytes of 8 rows an instruction, got 5.1).  Operands are read from 8 (K) or 4 (V) rows at a time; the
+// exclusive-or, together with the order in which tokens are assigned to operand rows (token_of), lets the eight (K,
+// V) or sixteen (V, 8 bytes) lanes of a phase hit different banks.
+template <int kD, int kChunk>
+__device__ __forceinline__ uint32_t place(int row, int c) {
+  if constexpr (kD == 64) return row * 64 + ((c ^ ((row >> 1) & 2)) << 4);
+  return (c >> 3) * (kChunk * 128) + row * 128 + (((c ^ row) & 7) << 4);
+}
+// token (of 8) at operand row i: any bijection is right, as P and V are permuted alike
+template <int kD>
+__device__ __forceinline__ int token_of(int i) {
+  if constexpr (kD == 64) return (i & 4) | ((0x2130 >> (4 * (i & 3))) & 3);  // 0 3 1 2, 4 7 5 6
+  return i ^ ((i & 1) << 2);                                                  // 0 5 2 7, 4 1 6 3
+}
 
 // part of a tile in the workspace: O [kRows][kD], then (max, sum) [kRows][2]
 template <int kRows, int kD>
@@ -225,11 +241,12 @@ __device__ __forceinline__ void store_row(const KvAttentionParams& p, const Seq&
   }
 }
 
-template <int kD, int kNT, int kChunk, int kStages>
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentionParams p) {
-  using S = Shape<kD, kNT, kChunk, kStages>;
+template <int kD, int kNT, int kSub>
+__global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kernel(const KvAttentionParams p) {
+  using S = Shape<kD, kNT, kSub>;
   using C = Cursor<S::kRows, S::kUnit>;
-  extern __shared__ uint4 smem[];
+  constexpr int kChunk = S::kChunk, kStages = S::kStages;
+  extern __shared__ __align__(128) char smem[];
   __shared__ long long sums[kWarps];
   __shared__ long long found_before;
   __shared__ int found_b;
@@ -240,28 +257,25 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
   float* parts = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + p.parts_offset);
 
   // ---- this CTA's run of units
-  long long mine = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) mine += units_of<S::kRows, S::kUnit>(p, b);
+  if (threadIdx.x == 0) splits[cta].last_cta = -1;
+  long long total = 0, own = 0;
+  for (int b = threadIdx.x; b < p.batch; b += kThreads) own = units_of<S::kRows, S::kUnit>(p, b), total += own;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) sums[warp] = total;
   __syncthreads();
-  long long total = 0;
+  total = sums[0];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += sums[w];
+  for (int w = 1; w < kWarps; ++w) total += sums[w];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid to complete
   // no more CTAs than units: every one of them then has a part in what it touches, which the join relies on
   const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
-  const long long run_begin = cta < ctas ? total * cta / ctas : total;
-  const long long run_end = cta < ctas ? total * (cta + 1) / ctas : total;
-  if (run_begin >= run_end) {
-    if (threadIdx.x == 0) splits[cta].last_cta = -1;
-    return;
-  }
+  if (cta >= ctas) return;
+  const long long run_begin = total * cta / ctas, run_end = total * (cta + 1) / ctas;
   long long before = 0;  // units of the sequences in front of b0
   for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    const long long own = b < p.batch ? units_of<S::kRows, S::kUnit>(p, b) : 0;
+    if (p.batch > kThreads) own = b < p.batch ? units_of<S::kRows, S::kUnit>(p, b) : 0;  // else it is there already
     long long upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -299,56 +313,77 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
   C ahead = cur;
   long long ahead_at = run_begin;
 
-  // ---- the ring: each lane copies what it will read
-  const uint32_t ring = smem_addr(smem) + static_cast<uint32_t>(warp * kStages * S::kStageBytes);
-  const uint32_t k_off = lane * 16;
-  const uint32_t v_off = 32 * 16 * S::kKVecs + lane * S::kVBytes;
-  const uint32_t s_off = 32 * (16 * S::kKVecs + S::kVBytes * S::kVVecs) + lane * 8;
-  float* merge = reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + S::kRingBytes);
-  float* merge_ml = merge + kWarps * S::kRows * S::kPitch;
+  // ---- the ring of a warp: it copies and reads its own chunks, in step
+  char* const ring = smem + warp * kStages * S::kStageBytes;
+  constexpr int kRowVecs = kD / 16;         // 16-byte vectors of a row
+  constexpr int kCopyRows = 32 / kRowVecs;  // rows that one copy instruction of the warp covers
+  const int copy_row = lane / kRowVecs, copy_vec = lane % kRowVecs;
+  // operand rows: K tokens g and g + 8 of 16; V tokens 2t, 2t + 1 and those + 8 (the placement repeats after 8 rows)
+  int k_at[kD / 64], v_at[2][S::kVH];
+#pragma unroll
+  for (int j = 0; j < kD / 64; ++j) k_at[j] = place<kD, kChunk>(token_of<kD>(g), 4 * j + t);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < S::kVH; ++h) {
+      const int row = token_of<kD>(2 * t + i);
+      v_at[i][h] = S::kTileBytes + (kD == 64 ? place<kD, kChunk>(row, g >> 1) + 8 * (g & 1) : place<kD, kChunk>(row, 8 * h + g));
+    }
+  constexpr int k8Rows = 8 * (kD == 64 ? 64 : 128);  // bytes from a row to the one 8 further
+  __shared__ float join_ml[kWarps][S::kRows][2];
+  __shared__ __align__(8) float row_scale[S::kRows];  // of a query row: what its scores are multiplied by, in units of log2
+  __shared__ __align__(8) int row_end[S::kRows];      // the tokens it sees: [0, end)
+  char* const queries = smem + S::kRingBytes;
 
-  int next_page = -1;  // page of the chunk that is requested next, loaded one step early
+  int next_page = -1;  // lane i: page of part i of the chunk that is requested next, loaded one step early
   const auto look_up = [&]() {
     next_page = -1;
-    if (ahead_at < run_end) {
-      const int token0 = ahead.unit * S::kUnit + warp * kChunk;
-      if (token0 < ahead.max_end) next_page = p.block_table[ahead.b * p.bt_stride + (token0 >> p.page_shift)];
+    if (ahead_at < run_end && lane < S::kSubs) {
+      const int token = ahead.unit * S::kUnit + warp * kChunk + lane * kSub;
+      if (token < ahead.max_end) next_page = p.block_table[ahead.b * p.bt_stride + (token >> p.page_shift)];
     }
   };
   const auto request = [&](int stage) {  // one group a call, also when there is nothing to request
     if (ahead_at < run_end) {
       const int token0 = ahead.unit * S::kUnit + warp * kChunk;
       if (token0 < ahead.max_end) {
-        const uint32_t base = ring + stage * S::kStageBytes;
-        const bool there = next_page >= 0 && next_page < p.num_pages;
-        const long long page = there ? next_page : 0;
-        const int row0 = token0 & (p.page_size - 1);
-        const uint8_t* k = p.k_cache + page * p.k_page + ahead.kv_head * p.k_head + row0 * p.k_row;
-        const uint8_t* v = p.v_cache + page * p.v_page + ahead.kv_head * p.v_head + row0 * p.v_row;
+        char* const at = ring + stage * S::kStageBytes;
+        const uint32_t base = smem_addr(at);
+        const int mine = next_page >= 0 && next_page < p.num_pages ? next_page : -1;
 #pragma unroll
-        for (int i = 0; i < kChunk / 8; ++i) {
-          const bool take = there && token0 + 8 * i + g < ahead.max_end;
-          const uint8_t* row = k + (8 * i + g) * p.k_row + 16 * t;
+        for (int sub = 0; sub < S::kSubs; ++sub) {
+          const int page = __shfl_sync(0xffffffffu, mine, sub);
+          const long long at_page = max(page, 0);
+          const int row0 = ((token0 + sub * kSub) & (p.page_size - 1)) + copy_row;
+          const uint8_t* k = p.k_cache + at_page * p.k_page + ahead.kv_head * p.k_head + row0 * p.k_row + 16 * copy_vec;
+          const uint8_t* v = p.v_cache + at_page * p.v_page + ahead.kv_head * p.v_head + row0 * p.v_row + 16 * copy_vec;
+          const int left = page < 0 ? 0 : ahead.max_end - token0 - sub * kSub;  // tokens of the part that there are
+          if (left >= kSub) {
 #pragma unroll
-          for (int j = 0; j < kD / 64; ++j) {
-            copy_async<16>(base + k_off + (i * (kD / 64) + j) * 512, take ? row + 64 * j : p.k_cache, take);
+            for (int i = 0; i < kSub; i += kCopyRows) {
+              const uint32_t to = base + place<kD, kChunk>(sub * kSub + i + copy_row, copy_vec);
+              copy_async<16>(to, k + i * p.k_row);
+              copy_async<16>(to + S::kTileBytes, v + i * p.v_row);
+            }
+          } else {  // zeros in place of the others: zero times NaN is NaN
+#pragma unroll
+            for (int i = 0; i < kSub; i += kCopyRows) {
+              const uint32_t to = base + place<kD, kChunk>(sub * kSub + i + copy_row, copy_vec);
+              const bool take = i + copy_row < left;
+              copy_async<16, false>(to, take ? k + i * p.k_row : p.k_cache, take);
+              copy_async<16, false>(to + S::kTileBytes, take ? v + i * p.v_row : p.v_cache, take);
+            }
           }
         }
-#pragma unroll
-        for (int i = 0; i < kChunk / 4; ++i) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
-          const int token = 16 * (i / 4) + 2 * t + (i & 1) + 8 * ((i >> 1) & 1);
-          const bool take = there && token0 + token < ahead.max_end;
-          const uint8_t* row = v + token * p.v_row + S::kVBytes * g;
-#pragma unroll
-          for (int h = 0; h < S::kVH; ++h) {
-            copy_async<S::kVBytes>(base + v_off + (i * S::kVH + h) * 32 * S::kVBytes, take ? row + 128 * h : p.v_cache, take);
+        const int page = __shfl_sync(0xffffffffu, mine, lane >> 1);
+        if (lane < 2 * S::kSubs) {
+          if (page < 0) {
+            *reinterpret_cast<uint32_t*>(at + 2 * S::kTileBytes + 4 * lane) = kNoPage;
+          } else {
+            copy_async<4>(base + 2 * S::kTileBytes + 4 * lane,
+                          (lane & 1) ? p.v_scale + page * p.vs_page + ahead.kv_head * p.vs_head
+                                     : p.k_scale + page * p.ks_page + ahead.kv_head * p.ks_head);
           }
-        }
-        if (there) {
-          copy_async<4>(base + s_off, p.k_scale + page * p.ks_page + ahead.kv_head * p.ks_head, true);
-          copy_async<4>(base + s_off + 4, p.v_scale + page * p.vs_page + ahead.kv_head * p.vs_head, true);
-        } else {
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + s_off), "r"(kNoPage) : "memory");
         }
       }
       ++ahead_at;
@@ -363,100 +398,105 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
 
   int stage = 0;
   long long at = run_begin;
-  if (threadIdx.x == 0) splits[cta].last_cta = -1;
   while (at < run_end) {
     // ---- a segment: the units of this run that belong to one tile
     const int unit0 = cur.unit;
     const int unit_end = static_cast<int>(min(static_cast<long long>(cur.s.units), unit0 + (run_end - at)));
     const int rows = min(S::kRows, cur.s.n * p.group - cur.row0);
-    // queries: column 8 nt + g, elements 64 j + 16 t .. + 15
-    uint32_t qf[kNT][kD / 64][8];
-    float col_scale[kNT][2];
-    int col_end[kNT][2];
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      const int r = 8 * nt + g;
-      float x[kD / 64][16];
-      float big = 0.0f;
-      const bool real = r < rows;
-      const int row = cur.row0 + (real ? r : 0);
+    // queries to fp16, each row scaled by a power of two to a largest element in [1, 2); 16 elements a thread
+    for (int i = threadIdx.x; i < S::kRows * (kD / 16); i += kThreads) {
+      const int r = i / (kD / 16), piece = i % (kD / 16);
+      const int row = cur.row0 + min(r, rows - 1);
       const int token = row / p.group;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + (cur.s.q_base + static_cast<long long>(token)) * p.q_token +
-                          (cur.kv_head * p.group + row - token * p.group) * p.q_head + 16 * t;
-#pragma unroll
-      for (int j = 0; j < kD / 64; ++j) {
-        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-        if (real) {
-          lo = *reinterpret_cast<const uint4*>(q + 64 * j);
-          hi = *reinterpret_cast<const uint4*>(q + 64 * j + 8);
-        }
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (cur.s.q_base + static_cast<long long>(token)) * p.q_token +
+                                                      (cur.kv_head * p.group + row - token * p.group) * p.q_head + 16 * piece);
+      float x[16], big = 0.0f;
+      {
         float a[8], b[8];
-        unpack_q(lo, p.fp16, a);
-        unpack_q(hi, p.fp16, b);
+        unpack_q(q[0], p.fp16, a);
+        unpack_q(q[1], p.fp16, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[j][i] = a[i];
-          x[j][8 + i] = b[i];
-          big = fmaxf(big, fmaxf(fabsf(a[i]), fabsf(b[i])));
+        for (int e = 0; e < 8; ++e) {
+          x[e] = a[e];
+          x[8 + e] = b[e];
+          big = fmaxf(big, fmaxf(fabsf(a[e]), fabsf(b[e])));
         }
       }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // 2^-e with the row's largest element in [1, 2); rows of zeros, and with infinities, as they are
+#pragma unroll
+      for (int o = 1; o < kD / 16; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      // rows of zeros, and with infinities, as they are
       int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
       e = big > 0.0f && e < 128 ? max(min(e, 126), -126) : 0;
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      if (p.softmax_scale < 0.0f) down = -down;  // the factor on the scores stays positive: their maximum is found first
+      uint32_t h[8];
 #pragma unroll
-      for (int j = 0; j < kD / 64; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[nt][j][i] = half2_of(x[j][2 * i] * down, x[j][2 * i + 1] * down);
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        col_scale[nt][c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4) * (p.softmax_scale * kLog2e);
-        const int rc = 8 * nt + 2 * t + c;
-        col_end[nt][c] = rc < rows ? cur.s.len - cur.s.n + (cur.row0 + rc) / p.group + 1 : 0;
+      for (int c = 0; c < 8; ++c) h[c] = half2_of(x[2 * c] * down, x[2 * c + 1] * down);
+      uint4* to = reinterpret_cast<uint4*>(queries + r * kD * 2);
+      to[(2 * piece) ^ (r & 1)] = make_uint4(h[0], h[1], h[2], h[3]);  // neighbouring rows in different banks
+      to[(2 * piece + 1) ^ (r & 1)] = make_uint4(h[4], h[5], h[6], h[7]);
+      if (piece == 0) {
+        row_scale[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (fabsf(p.softmax_scale) * kLog2e);
+        row_end[r] = r < rows ? cur.s.len - cur.s.n + token + 1 : 0;
       }
     }
-    float o[S::kVH][kD >= 128 ? 8 : 4][kNT][4];
-    constexpr int kOT = kD >= 128 ? 8 : 4;  // 16-row tiles of O^T per vector of V
+    __syncthreads();
+    float o[S::kVH][S::kOT][kNT][4];
 #pragma unroll
     for (int h = 0; h < S::kVH; ++h)
 #pragma unroll
-      for (int i = 0; i < kOT; ++i)
+      for (int i = 0; i < S::kOT; ++i)
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[h][i][nt][c] = 0.0f;
+        for (int nt = 0; nt < kNT; ++nt) o[h][i][nt][0] = o[h][i][nt][1] = o[h][i][nt][2] = o[h][i][nt][3] = 0.0f;
+    float v_unit = 1.0f, v_top = 0.0f;  // unit of o, largest unit so far
     float m[kNT][2], l[kNT][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
+      m[nt][0] = m[nt][1] = kMinusInf;
       l[nt][0] = l[nt][1] = 0.0f;
     }
 
     for (int unit = unit0; unit < unit_end; ++unit) {
-      request(stage == 0 ? kStages - 1 : stage - 1);  // into the stage that was emptied one step ago
+      __syncwarp();                                   // all lanes have read the stage that was emptied one step ago
+      request(stage == 0 ? kStages - 1 : stage - 1);  // and is filled again
       copy_wait<kStages - 1>();
-      const uint32_t base = ring + stage * S::kStageBytes;
+      __syncwarp();  // what the other lanes copied is there too
+      const char* const base = ring + stage * S::kStageBytes;
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const int token0 = unit * S::kUnit + warp * kChunk;
       if (token0 >= cur.max_end) continue;
-      const uint2 sc = lds8(base + s_off);
-      if (sc.x == kNoPage) continue;
-      const float k_scale = __uint_as_float(sc.x), v_scale = __uint_as_float(sc.y);
+      float k_scale[S::kSubs], v_scale[S::kSubs];
+      bool there[S::kSubs];
+      bool partial = token0 + kChunk > cur.min_end;  // some column does not see all of the chunk
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) {
+        const uint2 sc = *reinterpret_cast<const uint2*>(base + 2 * S::kTileBytes + 8 * sub);
+        there[sub] = sc.x != kNoPage;
+        k_scale[sub] = __uint_as_float(sc.x);
+        v_scale[sub] = __uint_as_float(sc.y);
+        partial = partial || !there[sub];
+      }
 
       // ---- S^T = K Q^T
       float s[S::kMT][kNT][4];
 #pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt) {
+      for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kD / 64; ++j) {
-          const uint4 ka = lds16(base + k_off + ((2 * mt) * (kD / 64) + j) * 512);
-          const uint4 kb = lds16(base + k_off + ((2 * mt + 1) * (kD / 64) + j) * 512);
+      for (int j = 0; j < kD / 64; ++j) {
+        uint32_t qf[kNT][8];  // elements 64 j + 16 t .. + 15 of column 8 nt + g
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          const uint4* q = reinterpret_cast<const uint4*>(queries + (8 * nt + g) * kD * 2) + 8 * j;
+          const uint4 lo = q[(2 * t) ^ (g & 1)], hi = q[(2 * t + 1) ^ (g & 1)];
+          qf[nt][0] = lo.x, qf[nt][1] = lo.y, qf[nt][2] = lo.z, qf[nt][3] = lo.w;
+          qf[nt][4] = hi.x, qf[nt][5] = hi.y, qf[nt][6] = hi.z, qf[nt][7] = hi.w;
+        }
+#pragma unroll
+        for (int mt = 0; mt < S::kMT; ++mt) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(base + k_at[j] + 2 * mt * k8Rows);
+          const uint4 kb = *reinterpret_cast<const uint4*>(base + k_at[j] + (2 * mt + 1) * k8Rows);
           const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -464,31 +504,44 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
             halves_of(wa[i], a0, a2);
             halves_of(wb[i], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) mma16816(s[mt][nt], a0, a1, a2, a3, qf[nt][j][2 * i], qf[nt][j][2 * i + 1]);
+            for (int nt = 0; nt < kNT; ++nt) mma16816(s[mt][nt], a0, a1, a2, a3, qf[nt][2 * i], qf[nt][2 * i + 1]);
           }
         }
       }
       // ---- softmax over the tokens, column by column
-      const bool partial = token0 + kChunk > cur.min_end;
       float alpha[kNT][2];
       uint32_t pf[S::kMT][kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        const float f0 = col_scale[nt][0] * k_scale, f1 = col_scale[nt][1] * k_scale;
-        float top0 = m[nt][0], top1 = m[nt][1];
+        const float2 col = *reinterpret_cast<const float2*>(&row_scale[8 * nt + 2 * t]);
+        // Scores of one page: the factor goes into the exponent's argument (it is not negative, so the largest product is
+        // the largest score).  Scores of several pages, or masked ones, are multiplied first.
+        float e0 = col.x * k_scale[0], e1 = col.y * k_scale[0];
+        if (S::kSubs > 1 || partial) {
 #pragma unroll
-        for (int mt = 0; mt < S::kMT; ++mt) {
-          s[mt][nt][0] *= f0;
-          s[mt][nt][1] *= f1;
-          s[mt][nt][2] *= f0;
-          s[mt][nt][3] *= f1;
-          if (partial) {
-            const int token = token0 + 16 * mt + g;
-            if (token >= col_end[nt][0]) s[mt][nt][0] = __int_as_float(0xff800000);
-            if (token >= col_end[nt][1]) s[mt][nt][1] = __int_as_float(0xff800000);
-            if (token + 8 >= col_end[nt][0]) s[mt][nt][2] = __int_as_float(0xff800000);
-            if (token + 8 >= col_end[nt][1]) s[mt][nt][3] = __int_as_float(0xff800000);
+          for (int mt = 0; mt < S::kMT; ++mt) {
+            const float f0 = col.x * k_scale[mt * 16 / kSub], f1 = col.y * k_scale[mt * 16 / kSub];
+            s[mt][nt][0] *= f0;
+            s[mt][nt][1] *= f1;
+            s[mt][nt][2] *= f0;
+            s[mt][nt][3] *= f1;
           }
+          e0 = e1 = 1.0f;
+        }
+        if (partial) {
+          const int2 end = *reinterpret_cast<const int2*>(&row_end[8 * nt + 2 * t]);
+#pragma unroll
+          for (int mt = 0; mt < S::kMT; ++mt) {
+            const int token = there[mt * 16 / kSub] ? token0 + 16 * mt + token_of<kD>(g) : 0x7ffffff0;
+            if (token >= end.x) s[mt][nt][0] = kMinusInf;
+            if (token >= end.y) s[mt][nt][1] = kMinusInf;
+            if (token + 8 >= end.x) s[mt][nt][2] = kMinusInf;
+            if (token + 8 >= end.y) s[mt][nt][3] = kMinusInf;
+          }
+        }
+        float top0 = fmaxf(s[0][nt][0], s[0][nt][2]), top1 = fmaxf(s[0][nt][1], s[0][nt][3]);
+#pragma unroll
+        for (int mt = 1; mt < S::kMT; ++mt) {
           top0 = fmaxf(top0, fmaxf(s[mt][nt][0], s[mt][nt][2]));
           top1 = fmaxf(top1, fmaxf(s[mt][nt][1], s[mt][nt][3]));
         }
@@ -497,9 +550,11 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
           top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
           top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
         }
+        top0 = fmaxf(m[nt][0], top0 * e0);
+        top1 = fmaxf(m[nt][1], top1 * e1);
         // a column without a token so far: any finite reference will do
-        const float ref0 = top0 == __int_as_float(0xff800000) ? 0.0f : top0;
-        const float ref1 = top1 == __int_as_float(0xff800000) ? 0.0f : top1;
+        const float ref0 = top0 == kMinusInf ? 0.0f : top0;
+        const float ref1 = top1 == kMinusInf ? 0.0f : top1;
         alpha[nt][0] = exp2_approx(m[nt][0] - ref0);
         alpha[nt][1] = exp2_approx(m[nt][1] - ref1);
         m[nt][0] = top0;
@@ -507,8 +562,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
-          const float p0 = exp2_approx(s[mt][nt][0] - ref0), p1 = exp2_approx(s[mt][nt][1] - ref1);
-          const float p2 = exp2_approx(s[mt][nt][2] - ref0), p3 = exp2_approx(s[mt][nt][3] - ref1);
+          const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
+          const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
           sum0 += p0 + p2;
           sum1 += p1 + p3;
           pf[mt][nt][0] = transpose8x8(half2_of(p0, p1));
@@ -517,28 +572,44 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
         l[nt][0] = l[nt][0] * alpha[nt][0] + sum0;
         l[nt][1] = l[nt][1] * alpha[nt][1] + sum1;
       }
-      // ---- O^T += V^T P^T.  `end`: V counts as zero from this token on (kChunk and more: all of it counts)
-      const auto product = [&](auto cut, int end, auto takes) {
+      bool strange = false;
+      if (partial && cur.min_end < cur.max_end) {
+        // Tokens of this chunk that some columns see and others do not: their p is zero there, but zero times NaN is
+        // NaN.  Look whether such a token has a NaN (or its page a scale that is not finite).
+        bool bad = false;
+#pragma unroll
+        for (int sub = 0; sub < S::kSubs; ++sub) bad = bad || (there[sub] && !(fabsf(v_scale[sub]) <= kMaxFloat));
+#pragma unroll 1
+        for (int i = lane * 16; i < S::kTileBytes; i += 512) {
+          const uint4 v = *reinterpret_cast<const uint4*>(base + S::kTileBytes + i);
+          bad = bad || has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w);
+        }
+        strange = __any_sync(0xffffffffu, bad);
+      }
+      // ---- O^T += V^T P^T over one part of the chunk.  Plain: the products are added to O as they are.  cut: V counts as
+      // zero from token `end` of the chunk on, and the columns that `takes` names get f * product.
+      const auto product = [&](auto cut, int sub, int end, float f, auto takes) {
 #pragma unroll
         for (int h = 0; h < S::kVH; ++h) {
-          constexpr int kW = S::kVBytes / 4;
-          uint32_t w[S::kMT][4][kW];
+          constexpr int kW = S::kVW, kSteps = kSub / 16;
+          uint32_t w[kSteps][4][kW];
 #pragma unroll
-          for (int mt = 0; mt < S::kMT; ++mt)
+          for (int ks = 0; ks < kSteps; ++ks)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t a = base + v_off + ((4 * mt + i) * S::kVH + h) * 32 * S::kVBytes;
+              const int mt = sub * kSteps + ks;
+              const char* from = base + v_at[i & 1][h] + (2 * mt + (i >> 1)) * k8Rows;
               if constexpr (kW == 4) {
-                const uint4 v = lds16(a);
-                w[mt][i][0] = v.x, w[mt][i][1] = v.y, w[mt][i][2] = v.z, w[mt][i][3] = v.w;
+                const uint4 v = *reinterpret_cast<const uint4*>(from);
+                w[ks][i][0] = v.x, w[ks][i][1] = v.y, w[ks][i][2] = v.z, w[ks][i][3] = v.w;
               } else {
-                const uint2 v = lds8(a);
-                w[mt][i][0] = v.x, w[mt][i][1] = v.y;
+                const uint2 v = *reinterpret_cast<const uint2*>(from);
+                w[ks][i][0] = v.x, w[ks][i][1] = v.y;
               }
-              if constexpr (decltype(cut)::value) {
-                if (16 * mt + 2 * t + (i & 1) + 8 * (i >> 1) >= end) {
+              if constexpr (cut.value) {
+                if (16 * mt + token_of<kD>(2 * t + (i & 1)) + 8 * (i >> 1) >= end) {
 #pragma unroll
-                  for (int c = 0; c < kW; ++c) w[mt][i][c] = 0u;
+                  for (int c = 0; c < kW; ++c) w[ks][i][c] = 0u;
                 }
               }
             }
@@ -546,122 +617,157 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
           for (int c = 0; c < kW; ++c) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
+              float(&acc)[kNT][4] = o[h][2 * c + half];
               float d[kNT][4];
 #pragma unroll
               for (int nt = 0; nt < kNT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.0f;
 #pragma unroll
-              for (int mt = 0; mt < S::kMT; ++mt) {
+              for (int ks = 0; ks < kSteps; ++ks) {
                 const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;  // bytes 2 half, 2 half + 1 of two tokens, interleaved
+                const int mt = sub * kSteps + ks;
                 uint32_t a0, a1, a2, a3;
-                halves_of(__byte_perm(w[mt][0][c], w[mt][1][c], pick), a0, a1);
-                halves_of(__byte_perm(w[mt][2][c], w[mt][3][c], pick), a2, a3);
+                halves_of(__byte_perm(w[ks][0][c], w[ks][1][c], pick), a0, a1);
+                halves_of(__byte_perm(w[ks][2][c], w[ks][3][c], pick), a2, a3);
 #pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) mma16816(d[nt], a0, a1, a2, a3, pf[mt][nt][0], pf[mt][nt][1]);
+                for (int nt = 0; nt < kNT; ++nt) mma16816(cut.value ? d[nt] : acc[nt], a0, a1, a2, a3, pf[mt][nt][0], pf[mt][nt][1]);
               }
+              if constexpr (cut.value) {
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
+                for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float& acc = o[h][2 * c + half][nt][e];
-                  if (takes(nt, e & 1)) acc = fmaf(acc, alpha[nt][e & 1], d[nt][e] * v_scale);
-                }
+                  for (int e = 0; e < 4; ++e) {
+                    if (takes(nt, e & 1)) acc[nt][e] = fmaf(d[nt][e], f, acc[nt][e]);
+                  }
+              }
             }
           }
         }
       };
-      bool strange = false;
-      if (partial && cur.min_end < cur.max_end) {
-        // Tokens of this chunk that some columns see and others do not: their p is zero there, but zero times NaN is
-        // NaN.  Look whether such a token has a NaN (or its page a scale that is not finite).
-        bool bad = !(fabsf(v_scale) <= 3.402823466e38f);
+      // O is kept in units of the V scale of the page that was added last, so that products can be added to it where they
+      // are: O moves to a new unit together with the rescaling that a new maximum asks for, and mostly neither changes.
+      // A scale that is zero, not finite or 2^80 below the largest so far would take O out of fp32's range; such a part
+      // is multiplied on its own and added with its factor.
+      bool rescale = false;  // by alpha
 #pragma unroll
-        for (int i = 0; i < S::kVVecs; ++i) {
-          const uint32_t a = base + v_off + i * 32 * S::kVBytes;
-          const uint2 v = lds8(a);
-          bad |= has_nan_code(v.x) || has_nan_code(v.y);
-          if constexpr (S::kVBytes == 16) {
-            const uint2 u = lds8(a + 8);
-            bad |= has_nan_code(u.x) || has_nan_code(u.y);
+      for (int nt = 0; nt < kNT; ++nt) rescale = rescale || alpha[nt][0] != 1.0f || alpha[nt][1] != 1.0f;
+      rescale = __any_sync(0xffffffffu, rescale);
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) {
+        if (!there[sub]) continue;
+        const float vs = v_scale[sub];
+        const bool plain = !strange && vs <= kMaxFloat && vs > 0.0f && vs >= v_top * 0x1p-80f;
+        float ratio = 1.0f;
+        if (plain && vs != v_unit) {
+          if (v_top > 0.0f) ratio = __fdividef(v_unit, vs);
+          v_unit = vs;
+        }
+        if (plain) v_top = fmaxf(v_top, vs);
+        if (rescale || ratio != 1.0f) {
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            const float f0 = rescale ? alpha[nt][0] * ratio : ratio, f1 = rescale ? alpha[nt][1] * ratio : ratio;
+#pragma unroll
+            for (int h = 0; h < S::kVH; ++h)
+#pragma unroll
+              for (int i = 0; i < S::kOT; ++i) {
+                o[h][i][nt][0] *= f0;
+                o[h][i][nt][1] *= f1;
+                o[h][i][nt][2] *= f0;
+                o[h][i][nt][3] *= f1;
+              }
+          }
+          rescale = false;
+        }
+        if (plain) {
+          product(std::false_type{}, sub, 0, 1.0f, [](int, int) { return true; });
+        } else {
+          // once for every place where a column's context can end in this part or behind it, with V cut there; columns
+          // that see nothing of the part take nothing from it
+          const int lo = min(max(cur.min_end - token0, 0), kChunk), hi = min(cur.max_end - token0, kChunk);
+          for (int end = max(lo, sub * kSub + 1); end <= hi; ++end) {
+            product(std::true_type{}, sub, end, vs / v_unit, [&](int nt, int c) {
+              return min(row_end[8 * nt + 2 * t + c] - token0, kChunk) == end;
+            });
           }
         }
-        strange = __any_sync(0xffffffffu, bad);
-      }
-      if (!strange) {
-        product(std::false_type{}, 0, [](int, int) { return true; });
-      } else {
-        // once for every place where a column's context can end in this chunk, with V cut there
-        const int lo = max(cur.min_end - token0, 0), hi = min(cur.max_end - token0, kChunk);
-        for (int end = lo; end <= hi; ++end) {
-          product(std::true_type{}, end, [&](int nt, int c) {
-            return end > 0 && min(max(col_end[nt][c] - token0, 0), kChunk) == end;
-          });
-        }
-        // columns that see nothing of the chunk keep their sums: alpha is one there, unless they have seen nothing yet
       }
     }
 
-    // ---- join the warps
+    // ---- join the warps: O in the stage that was emptied last (no copy into it is on its way), 16-byte vectors of a
+    // row exchanged so that the lanes of a phase write to different banks
+    const bool begins = unit0 == 0, ends = unit_end == cur.s.units;
+    float* const part = parts + (2ll * cta + (begins ? 1 : 0)) * part_floats<S::kRows, kD>();
+    const int last = stage == 0 ? kStages - 1 : stage - 1;  // the warps of a block are at the same stage
+    const auto join_row = [&](int w, int r) {
+      return reinterpret_cast<float4*>(smem + (w * kStages + last) * S::kStageBytes) + r * (kD / 4);
+    };
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
-        const int r = 8 * nt + 2 * t + c;
-        float* row = merge + (warp * S::kRows + r) * S::kPitch;
-#pragma unroll
-        for (int h = 0; h < S::kVH; ++h) {
-          constexpr int kPer = S::kVBytes;  // elements of the head dimension that a lane has in a row
-          float* d = row + 128 * h + kPer * g;
-#pragma unroll
-          for (int i = 0; i < kOT; i += 2) {
-            *reinterpret_cast<float4*>(d + 2 * i) =
-                make_float4(o[h][i][nt][c], o[h][i][nt][2 + c], o[h][i + 1][nt][c], o[h][i + 1][nt][2 + c]);
-          }
-        }
         if (g == 0) {
-          merge_ml[(warp * S::kRows + r) * 2] = m[nt][c];
-          merge_ml[(warp * S::kRows + r) * 2 + 1] = l[nt][c];
+          join_ml[warp][8 * nt + 2 * t + c][0] = m[nt][c];
+          join_ml[warp][8 * nt + 2 * t + c][1] = l[nt][c];
         }
       }
-    __syncthreads();
-    const bool begins = unit0 == 0, ends = unit_end == cur.s.units;
-    float* part = parts + (2ll * cta + (begins ? 1 : 0)) * part_floats<S::kRows, kD>();
-    for (int i = threadIdx.x; i < rows * (kD / 4); i += kThreads) {
-      const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
-      float top = merge_ml[r * 2];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, merge_ml[(w * S::kRows + r) * 2]);
-      const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float sum = 0.0f;
+    for (int nt0 = 0; nt0 < kNT; nt0 += S::kJoinNT) {
+      if (nt0 > 0) __syncthreads();  // the rows before have been read
+      __syncwarp();                  // all lanes have read the stage
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_approx(merge_ml[(w * S::kRows + r) * 2] - ref);
-        const float4 v = *reinterpret_cast<const float4*>(merge + (w * S::kRows + r) * S::kPitch + d);
-        sum = fmaf(merge_ml[(w * S::kRows + r) * 2 + 1], f, sum);
-        acc.x = fmaf(v.x, f, acc.x);
-        acc.y = fmaf(v.y, f, acc.y);
-        acc.z = fmaf(v.z, f, acc.z);
-        acc.w = fmaf(v.w, f, acc.w);
-      }
-      if (begins && ends) {
-        store_row(p, cur.s, cur.kv_head, cur.row0 + r, d, acc, top, sum);
-      } else {
-        *reinterpret_cast<float4*>(part + r * kD + d) = acc;
-        if (d == 0) {
-          part[S::kRows * kD + 2 * r] = top;
-          part[S::kRows * kD + 2 * r + 1] = sum;
+      for (int nt = nt0; nt < nt0 + S::kJoinNT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float4* row = join_row(warp, 8 * (nt - nt0) + 2 * t + c);
+#pragma unroll
+          for (int h = 0; h < S::kVH; ++h)
+#pragma unroll
+            for (int i = 0; i < S::kOT; i += 2) {
+              row[(32 * h + S::kVW * g + i / 2) ^ t] =
+                  make_float4(o[h][i][nt][c] * v_unit, o[h][i][nt][2 + c] * v_unit, o[h][i + 1][nt][c] * v_unit,
+                              o[h][i + 1][nt][2 + c] * v_unit);
+            }
+        }
+      __syncthreads();
+      const int first_row = 8 * nt0, row_count = min(rows - first_row, 8 * S::kJoinNT);
+      for (int i = threadIdx.x; i < row_count * (kD / 4); i += kThreads) {
+        const int in = i / (kD / 4), d = i % (kD / 4), r = first_row + in;
+        float top = join_ml[0][r][0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_ml[w][r][0]);
+        const float ref = top == kMinusInf ? 0.0f : top;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2_approx(join_ml[w][r][0] - ref);
+          const float4 v = join_row(w, in)[d ^ ((r >> 1) & 3)];
+          sum = fmaf(join_ml[w][r][1], f, sum);
+          acc.x = fmaf(v.x, f, acc.x);
+          acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z);
+          acc.w = fmaf(v.w, f, acc.w);
+        }
+        if (begins && ends) {
+          store_row(p, cur.s, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum);
+        } else {
+          reinterpret_cast<float4*>(part)[r * (kD / 4) + d] = acc;
+          if (d == 0) {
+            part[S::kRows * kD + 2 * r] = top;
+            part[S::kRows * kD + 2 * r + 1] = sum;
+          }
         }
       }
     }
     if (begins && !ends && threadIdx.x == 0) {
-      const long long tile_end = at + (cur.s.units - unit0);  // unit0 is 0: one past the tile's last unit
+      const long long tile_end = at + cur.s.units;  // one past the tile's last unit: the segment begins with its first
       splits[cta].last_cta = static_cast<int>((tile_end * ctas - 1) / total);
       splits[cta].b = cur.b;
       splits[cta].tile = cur.tile;
     }
-    __syncthreads();  // the warps' sums have been read
+    __syncthreads();  // the warps' sums and the queries have been read
     at += unit_end - unit0;
     cur.unit = unit_end - 1;
     cur.advance(p, run_end - at);
@@ -669,10 +775,15 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(const KvAttentio
   copy_wait<0>();
 }
 
-// Joins the parts of the tile that CTA blockIdx.x of the first kernel began and others finished.
-template <int kD, int kNT, int kChunk>
+// Joins the parts of the tile that CTA blockIdx.x of the first kernel began and others finished.  One long sequence
+// leaves a few tiles of many parts each: four groups of threads take every fourth part, kAhead loads in flight.
+constexpr int kJoinGroups = 4, kAhead = 4;
+
+template <int kD, int kNT, int kUnit>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const KvAttentionParams p) {
-  constexpr int kRows = 8 * kNT, kUnit = kWarps * kChunk;
+  constexpr int kRows = 8 * kNT, kVecs = kD / 4, kLanes = kJoinThreads / kJoinGroups;
+  __shared__ float4 sums[kJoinGroups - 1][kLanes];
+  __shared__ float weights[kJoinGroups - 1][kLanes];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Split* splits = static_cast<const Split*>(p.workspace);
   const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + p.parts_offset);
@@ -687,7 +798,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
       if (p.fill_rest) {
         for (int d = threadIdx.x; d < kD; d += kJoinThreads) o[d] = 0;
       }
-      if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.heads + head] = __int_as_float(0xff800000);
+      if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.heads + head] = kMinusInf;
     }
   }
   const Split sp = splits[cta];
@@ -699,27 +810,78 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   cur.enter_tile(p);
   const int rows = min(kRows, cur.s.n * p.group - cur.row0);
   const int count = sp.last_cta - cta + 1;
+  const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
   // the beginning of the tile is part 1 of this CTA, what follows is part 0 of the next ones
   const auto part = [&](int i) { return parts + (2ll * (cta + i) + (i == 0 ? 1 : 0)) * part_floats<kRows, kD>(); };
-  for (int i = threadIdx.x; i < rows * (kD / 4); i += kJoinThreads) {
-    const int r = i / (kD / 4), d = (i - r * (kD / 4)) * 4;
-    float top = __int_as_float(0xff800000);
-    for (int c = 0; c < count; ++c) top = fmaxf(top, part(c)[kRows * kD + 2 * r]);
-    const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
+  for (int first = 0; first < rows * kVecs; first += kLanes) {
+    const int i = first + lane;
+    const bool live = i < rows * kVecs;
+    const int r = live ? i / kVecs : 0, d = i % kVecs;
+    float top = kMinusInf, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < count; ++c) {
-      const float* x = part(c);
-      const float f = exp2_approx(x[kRows * kD + 2 * r] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(x + r * kD + d);
-      sum = fmaf(x[kRows * kD + 2 * r + 1], f, sum);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
+    for (int c0 = group; c0 < count; c0 += kJoinGroups * kAhead) {
+      float m[kAhead], l[kAhead];
+      float4 v[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int c = c0 + x * kJoinGroups;
+        m[x] = kMinusInf;
+        if (c < count && live) {
+          const float* at = part(c);
+          m[x] = at[kRows * kD + 2 * r];
+          l[x] = at[kRows * kD + 2 * r + 1];
+          v[x] = reinterpret_cast<const float4*>(at)[r * kVecs + d];
+        } else {
+          l[x] = 0.0f;
+          v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+      float ref = top;
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) ref = fmaxf(ref, m[x]);
+      const float base = ref == kMinusInf ? 0.0f : ref;
+      const float old = exp2_approx(top - base);
+      top = ref;
+      sum *= old;
+      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const float f = exp2_approx(m[x] - base);
+        sum = fmaf(l[x], f, sum);
+        acc.x = fmaf(v[x].x, f, acc.x);
+        acc.y = fmaf(v[x].y, f, acc.y);
+        acc.z = fmaf(v[x].z, f, acc.z);
+        acc.w = fmaf(v[x].w, f, acc.w);
+      }
     }
-    store_row(p, cur.s, cur.kv_head, cur.row0 + r, d, acc, top, sum);
+    __shared__ float tops[kJoinGroups - 1][kLanes];
+    if (group > 0) {
+      sums[group - 1][lane] = acc;
+      weights[group - 1][lane] = sum;
+      tops[group - 1][lane] = top;
+    }
+    __syncthreads();
+    if (group == 0 && live) {
+      float ref = top;
+#pragma unroll
+      for (int x = 0; x < kJoinGroups - 1; ++x) ref = fmaxf(ref, tops[x][lane]);
+      const float base = ref == kMinusInf ? 0.0f : ref;
+      const float old = exp2_approx(top - base);
+      sum *= old;
+      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+      for (int x = 0; x < kJoinGroups - 1; ++x) {
+        const float f = exp2_approx(tops[x][lane] - base);
+        const float4 v = sums[x][lane];
+        sum = fmaf(weights[x][lane], f, sum);
+        acc.x = fmaf(v.x, f, acc.x);
+        acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z);
+        acc.w = fmaf(v.w, f, acc.w);
+      }
+      store_row(p, cur.s, cur.kv_head, cur.row0 + r, 4 * d, acc, ref, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -729,9 +891,9 @@ struct Plan {
 };
 
 // CTAs of a grid that fills the current device once, per device (the same whoever asks first)
-template <int kD, int kNT, int kChunk, int kStages>
+template <int kD, int kNT, int kSub>
 cudaError_t make_plan(Plan* plan) {
-  using S = Shape<kD, kNT, kChunk, kStages>;
+  using S = Shape<kD, kNT, kSub>;
   static std::atomic<int> ctas_per_device[64] = {};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -739,7 +901,7 @@ cudaError_t make_plan(Plan* plan) {
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   int ctas = ctas_per_device[dev].load();
   if (ctas == 0) {
-    const auto kernel = kv_attention_kernel<kD, kNT, kChunk, kStages>;
+    const auto kernel = kv_attention_kernel<kD, kNT, kSub>;
     int sms = 0, per_sm = 0;
     err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (err != cudaSuccess) return err;
@@ -757,11 +919,11 @@ cudaError_t make_plan(Plan* plan) {
   return cudaSuccess;
 }
 
-template <int kD, int kNT, int kChunk, int kStages>
+template <int kD, int kNT, int kSub>
 cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t stream) {
-  using S = Shape<kD, kNT, kChunk, kStages>;
+  using S = Shape<kD, kNT, kSub>;
   Plan plan;
-  cudaError_t err = make_plan<kD, kNT, kChunk, kStages>(&plan);
+  cudaError_t err = make_plan<kD, kNT, kSub>(&plan);
   if (err != cudaSuccess) return err;
   if (bytes != nullptr) {  // only asked for the size
     *bytes = plan.bytes;
@@ -770,7 +932,7 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
   if (params.workspace_bytes < plan.bytes) return cudaErrorMemoryAllocation;
   KvAttentionParams p = params;
   p.parts_offset = plan.parts_offset;
-  kv_attention_kernel<kD, kNT, kChunk, kStages><<<plan.ctas, kThreads, S::kSmemBytes, stream>>>(p);
+  kv_attention_kernel<kD, kNT, kSub><<<plan.ctas, kThreads, S::kSmemBytes, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   // may be resident before the first kernel has ended; it waits for it (griddepcontrol.wait)
@@ -783,26 +945,26 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<kD, kNT, kChunk>, p);
+  return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<kD, kNT, S::kUnit>, p);
 }
 
-template <int kD>
-cudaError_t run_d(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream) {
+template <int kD, int kSub>
+cudaError_t run_rows(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream) {
   // query rows that share a kv head, in an average sequence
-  const long long rows = p.cu_seqlens == nullptr ? p.group : (static_cast<long long>(p.tokens) * p.group + p.batch - 1) / max(p.batch, 1);
-  const bool wide = rows > 8;
-  if (p.page_size >= 32) {
-    return wide ? run_t<kD, 2, 32, 2>(p, bytes, stream) : run_t<kD, 1, 32, 2>(p, bytes, stream);
+  const long long rows = p.cu_seqlens == nullptr ? p.group : (static_cast<long long>(p.tokens) * p.group + p.batch - 1) / (p.batch > 0 ? p.batch : 1);
+  if (rows <= 8) return run_t<kD, 1, kSub>(p, bytes, stream);
+  if constexpr (kD <= 128) {
+    if (rows > 16) return run_t<kD, 4, kSub>(p, bytes, stream);
   }
-  return wide ? run_t<kD, 2, 16, 3>(p, bytes, stream) : run_t<kD, 1, 16, 3>(p, bytes, stream);
+  return run_t<kD, 2, kSub>(p, bytes, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_attention(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream) {
-  if (p.dim == 64) return run_d<64>(p, bytes, stream);
-  if (p.dim == 128) return run_d<128>(p, bytes, stream);
-  return run_d<256>(p, bytes, stream);
+  if (p.dim == 64) return p.page_size >= 32 ? run_rows<64, 32>(p, bytes, stream) : run_rows<64, 16>(p, bytes, stream);
+  if (p.dim == 128) return p.page_size >= 32 ? run_rows<128, 32>(p, bytes, stream) : run_rows<128, 16>(p, bytes, stream);
+  return run_rows<256, 16>(p, bytes, stream);
 }
 
 }  // namespace b200fp8
