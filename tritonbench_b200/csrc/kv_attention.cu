@@ -35,7 +35,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMaxFloat = 3.402823466e38f;
@@ -124,13 +124,39 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionParams& p, int b) {
   s.units = max((s.len + kUnit - 1) / kUnit, 1);
   return s;
 }
+// Cost of a tile besides its units, in units: loading the queries, joining the warps and storing what they found takes a
+// block about 2.3 us, a unit takes it 2.0 us (three blocks an SM, the memory busy).  Runs of equal units without it ended
+// between 67 and 98 us (64 sequences of 1 to 8192 tokens), those with eleven tiles last.
+// With 32 rows (three times the join, two blocks an SM) a tile costs 3: 32 requests of 1 to 6 tokens 143 -> 129 us.
+template <int kRows>
+__host__ __device__ constexpr int tile_cost() { return kRows == 32 ? 3 : 1; }
+
 template <int kRows, int kUnit>
-__device__ __forceinline__ long long units_of(const KvAttentionParams& p, int b) {
+__device__ __forceinline__ long long cost_of(const KvAttentionParams& p, int b) {
   const Seq s = seq_of<kRows, kUnit>(p, b);
-  return static_cast<long long>(s.row_tiles) * p.kv_heads * s.units;
+  return static_cast<long long>(s.row_tiles) * p.kv_heads * (s.units + tile_cost<kRows>());
 }
 
-// A place in the list: unit `unit` of tile `tile` (kv head, row tile) of sequence b.
+// Equal shares of `total`: CTA c has [begin(c), begin(c + 1)).
+struct Shares {
+  long long each, rest;  // the first `rest` shares are one larger
+  __device__ __forceinline__ Shares(long long total, int ctas) {
+    if (total <= 0xffffffffll) {  // 64-bit division is slow
+      each = static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas);
+    } else {
+      each = total / ctas;
+    }
+    rest = total - each * ctas;
+  }
+  __device__ __forceinline__ long long begin(int c) const { return c * each + (c < rest ? c : rest); }
+  __device__ __forceinline__ int holder(long long at) const {  // CTA whose share `at` is in
+    const long long large = rest * (each + 1);
+    return static_cast<int>(at < large ? at / (each + 1) : rest + (at - large) / each);
+  }
+};
+
+// A place in the list: unit `unit` of tile `tile` (kv head, row tile) of sequence b.  The cost of a tile lies in front of
+// its units: a share that begins or ends there begins or ends with the tile's first unit.
 template <int kRows, int kUnit>
 struct Cursor {
   Seq s;
@@ -150,9 +176,12 @@ struct Cursor {
   __device__ __forceinline__ void enter_sequence(const KvAttentionParams& p) {
     s = seq_of<kRows, kUnit>(p, b);
   }
-  __device__ __forceinline__ void advance(const KvAttentionParams& p, long long left) {
-    if (++unit < s.units) return;
-    if (left <= 0) return;  // the run ends here
+  // To the next unit, `left` being the rest of the share behind the present one, which becomes what is left behind the
+  // cost of a tile that is entered.
+  __device__ __forceinline__ void advance(const KvAttentionParams& p, long long& left) {
+    if (++unit < s.units || left <= 0) return;
+    left -= tile_cost<kRows>();
+    if (left <= 0) return;  // the share ends in front of the tile's first unit
     unit = 0;
     if (++tile == s.row_tiles * p.kv_heads) {
       tile = 0;
@@ -208,9 +237,11 @@ __device__ __forceinline__ int token_of(int i) {
 template <int kRows, int kD>
 __host__ __device__ constexpr size_t part_floats() { return static_cast<size_t>(kRows) * (kD + 2); }
 
-struct Split {  // a tile that CTA c began and did not finish
-  int last_cta;  // the CTA that finishes it; -1: none
-  int b, tile;
+struct alignas(16) Split {  // of CTA c
+  int first_cta;  // the CTA that began the tile inside which the share of c begins; -1: none
+  int last_cta;   // the CTA that finishes the tile which c began and did not finish; -1: none.  Then, of that tile:
+  int q_base, kv_head, row0, rows;
+  int pad[2];
 };
 
 // q and out are bf16 or fp16: 16 bits an element either way
@@ -229,15 +260,15 @@ __device__ __forceinline__ uint32_t pack_out2(float lo, float hi, bool fp16) {
 }
 
 // Four elements of an output row from its sums, and the row's log-sum-exp (once, with the row's first elements).
-__device__ __forceinline__ void store_row(const KvAttentionParams& p, const Seq& s, int kv_head, int row, int d, float4 acc,
+__device__ __forceinline__ void store_row(const KvAttentionParams& p, int q_base, int kv_head, int row, int d, float4 acc,
                                           float top, float sum) {
   const int token = row / p.group;
   const int head = kv_head * p.group + row - token * p.group;
   const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);  // no token seen: zeros
-  uint16_t* at = static_cast<uint16_t*>(p.out) + (s.q_base + static_cast<long long>(token)) * p.o_token + head * p.o_head + d;
+  uint16_t* at = static_cast<uint16_t*>(p.out) + (q_base + static_cast<long long>(token)) * p.o_token + head * p.o_head + d;
   *reinterpret_cast<uint2*>(at) = make_uint2(pack_out2(acc.x * inv, acc.y * inv, p.fp16), pack_out2(acc.z * inv, acc.w * inv, p.fp16));
   if (p.lse != nullptr && d == 0) {
-    p.lse[(s.q_base + static_cast<long long>(token)) * p.heads + head] = (top + log2f(sum)) * kLn2;
+    p.lse[(q_base + static_cast<long long>(token)) * p.heads + head] = (top + log2f(sum)) * kLn2;
   }
 }
 
@@ -256,62 +287,83 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
   Split* splits = static_cast<Split*>(p.workspace);
   float* parts = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + p.parts_offset);
 
-  // ---- this CTA's run of units
-  if (threadIdx.x == 0) splits[cta].last_cta = -1;
+  // ---- this CTA's share of the list
+  if (threadIdx.x == 0) splits[cta].first_cta = splits[cta].last_cta = -1;
   long long total = 0, own = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) own = units_of<S::kRows, S::kUnit>(p, b), total += own;
+  for (int b = threadIdx.x; b < p.batch; b += kThreads) own = cost_of<S::kRows, S::kUnit>(p, b), total += own;
+  long long upto = total;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) sums[warp] = total;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
   __syncthreads();
-  total = sums[0];
+  total = 0;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) total += sums[w];
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid to complete
-  // no more CTAs than units: every one of them then has a part in what it touches, which the join relies on
   const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
   if (cta >= ctas) return;
-  const long long run_begin = total * cta / ctas, run_end = total * (cta + 1) / ctas;
-  long long before = 0;  // units of the sequences in front of b0
-  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-    const int b = b0 + static_cast<int>(threadIdx.x);
-    if (p.batch > kThreads) own = b < p.batch ? units_of<S::kRows, S::kUnit>(p, b) : 0;  // else it is there already
-    long long upto = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    __syncthreads();  // sums of the step before have been read
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    long long step = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) upto += sums[w];
-      step += sums[w];
-    }
-    upto += before;
-    if (run_begin >= upto - own && run_begin < upto) {  // one thread of one step
-      found_b = b;
+  const Shares shares(total, ctas);
+  const long long run_begin = shares.begin(cta), run_end = shares.begin(cta + 1);
+  if (p.batch <= kThreads) {  // a thread has one sequence, and what lies in front of it
+    if (run_begin >= upto - own && run_begin < upto) {
+      found_b = threadIdx.x;
       found_before = upto - own;
     }
-    before += step;
-    if (before > run_begin) break;
+  } else {
+    long long before = 0;  // in front of b0
+    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      own = b < p.batch ? cost_of<S::kRows, S::kUnit>(p, b) : 0;
+      upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      __syncthreads();  // sums of the step before have been read
+      if (lane == 31) sums[warp] = upto;
+      __syncthreads();
+      long long step = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += sums[w];
+        step += sums[w];
+      }
+      upto += before;
+      if (run_begin >= upto - own && run_begin < upto) {  // one thread of one step
+        found_b = b;
+        found_before = upto - own;
+      }
+      before += step;
+      if (before > run_begin) break;
+    }
   }
   __syncthreads();
 
+  constexpr int kTileCost = tile_cost<S::kRows>();
   C cur;
   cur.b = found_b;
   cur.enter_sequence(p);
+  long long left = run_end - run_begin;  // of the share, from cur's unit on
   {
     const long long in_seq = run_begin - found_before;
-    cur.tile = static_cast<int>(in_seq / cur.s.units);
-    cur.unit = static_cast<int>(in_seq - static_cast<long long>(cur.tile) * cur.s.units);
+    const int tile_cost = cur.s.units + kTileCost;
+    cur.tile = static_cast<int>(in_seq <= 0xffffffffll ? static_cast<uint32_t>(in_seq) / static_cast<uint32_t>(tile_cost) : in_seq / tile_cost);
+    const int in_tile = static_cast<int>(in_seq - static_cast<long long>(cur.tile) * tile_cost);
+    cur.unit = max(in_tile - kTileCost, 0);
+    left -= max(kTileCost - in_tile, 0);
   }
+  if (left <= 0) return;  // nothing but the cost of a tile
   cur.enter_tile(p);
+  if (threadIdx.x == 0 && cur.unit > 0) splits[cta].first_cta = shares.holder(run_begin - cur.unit);
   C ahead = cur;
-  long long ahead_at = run_begin;
+  long long ahead_left = left;
 
   // ---- the ring of a warp: it copies and reads its own chunks, in step
   char* const ring = smem + warp * kStages * S::kStageBytes;
@@ -338,13 +390,13 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
   int next_page = -1;  // lane i: page of part i of the chunk that is requested next, loaded one step early
   const auto look_up = [&]() {
     next_page = -1;
-    if (ahead_at < run_end && lane < S::kSubs) {
+    if (ahead_left > 0 && lane < S::kSubs) {
       const int token = ahead.unit * S::kUnit + warp * kChunk + lane * kSub;
       if (token < ahead.max_end) next_page = p.block_table[ahead.b * p.bt_stride + (token >> p.page_shift)];
     }
   };
   const auto request = [&](int stage) {  // one group a call, also when there is nothing to request
-    if (ahead_at < run_end) {
+    if (ahead_left > 0) {
       const int token0 = ahead.unit * S::kUnit + warp * kChunk;
       if (token0 < ahead.max_end) {
         char* const at = ring + stage * S::kStageBytes;
@@ -386,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
           }
         }
       }
-      ++ahead_at;
-      ahead.advance(p, run_end - ahead_at);
+      --ahead_left;
+      ahead.advance(p, ahead_left);
     }
     copy_commit();
     look_up();
@@ -397,11 +449,10 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
   for (int s = 0; s < kStages - 1; ++s) request(s);
 
   int stage = 0;
-  long long at = run_begin;
-  while (at < run_end) {
+  while (left > 0) {
     // ---- a segment: the units of this run that belong to one tile
     const int unit0 = cur.unit;
-    const int unit_end = static_cast<int>(min(static_cast<long long>(cur.s.units), unit0 + (run_end - at)));
+    const int unit_end = static_cast<int>(min(static_cast<long long>(cur.s.units), unit0 + left));
     const int rows = min(S::kRows, cur.s.n * p.group - cur.row0);
     // queries to fp16, each row scaled by a power of two to a largest element in [1, 2); 16 elements a thread
     for (int i = threadIdx.x; i < S::kRows * (kD / 16); i += kThreads) {
@@ -751,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
           acc.w = fmaf(v.w, f, acc.w);
         }
         if (begins && ends) {
-          store_row(p, cur.s, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum);
+          store_row(p, cur.s.q_base, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum);
         } else {
           reinterpret_cast<float4*>(part)[r * (kD / 4) + d] = acc;
           if (d == 0) {
@@ -762,28 +813,50 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
       }
     }
     if (begins && !ends && threadIdx.x == 0) {
-      const long long tile_end = at + cur.s.units;  // one past the tile's last unit: the segment begins with its first
-      splits[cta].last_cta = static_cast<int>((tile_end * ctas - 1) / total);
-      splits[cta].b = cur.b;
-      splits[cta].tile = cur.tile;
+      // the share ends with this segment, so the tile's last unit is as far behind the share's end as behind the segment's
+      splits[cta].last_cta = shares.holder(run_end + (cur.s.units - unit_end) - 1);
+      splits[cta].q_base = cur.s.q_base;
+      splits[cta].kv_head = cur.kv_head;
+      splits[cta].row0 = cur.row0;
+      splits[cta].rows = rows;
     }
     __syncthreads();  // the warps' sums and the queries have been read
-    at += unit_end - unit0;
+    left -= unit_end - unit0;
     cur.unit = unit_end - 1;
-    cur.advance(p, run_end - at);
+    cur.advance(p, left);
   }
   copy_wait<0>();
 }
 
-// Joins the parts of the tile that CTA blockIdx.x of the first kernel began and others finished.  One long sequence
-// leaves a few tiles of many parts each: four groups of threads take every fourth part, kAhead loads in flight.
-constexpr int kJoinGroups = 4, kAhead = 4;
+// Joins the parts of the tiles that several CTAs of the first kernel shared.  The blocks of the CTAs that shared a tile
+// share its join too (one long sequence leaves a few tiles of many parts each): each takes some of the output's 16-byte
+// vectors, with up to kGroups groups of threads that take every kGroups-th part, kAhead loads in flight.
+constexpr int kGroups = 8, kAhead = 4;
 
-template <int kD, int kNT, int kUnit>
+struct RunningSum {
+  float top, sum;
+  float4 acc;
+  __device__ __forceinline__ void move_to(float ref) {  // ref not below top
+    const float f = exp2_approx(top - (ref == kMinusInf ? 0.0f : ref));
+    top = ref;
+    sum *= f;
+    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+  }
+  __device__ __forceinline__ void add(float m, float l, float4 v) {  // m not above top
+    const float f = exp2_approx(m - (top == kMinusInf ? 0.0f : top));
+    sum = fmaf(l, f, sum);
+    acc.x = fmaf(v.x, f, acc.x);
+    acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z);
+    acc.w = fmaf(v.w, f, acc.w);
+  }
+};
+
+template <int kD, int kNT>
 __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const KvAttentionParams p) {
-  constexpr int kRows = 8 * kNT, kVecs = kD / 4, kLanes = kJoinThreads / kJoinGroups;
-  __shared__ float4 sums[kJoinGroups - 1][kLanes];
-  __shared__ float weights[kJoinGroups - 1][kLanes];
+  constexpr int kRows = 8 * kNT, kVecs = kD / 4;
+  __shared__ float4 group_acc[kJoinThreads];
+  __shared__ float2 group_ml[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Split* splits = static_cast<const Split*>(p.workspace);
   const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + p.parts_offset);
@@ -801,87 +874,63 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
       if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.heads + head] = kMinusInf;
     }
   }
-  const Split sp = splits[cta];
-  if (sp.last_cta < 0) return;
-  Cursor<kRows, kUnit> cur;
-  cur.b = sp.b;
-  cur.tile = sp.tile;
-  cur.enter_sequence(p);
-  cur.enter_tile(p);
-  const int rows = min(kRows, cur.s.n * p.group - cur.row0);
-  const int count = sp.last_cta - cta + 1;
-  const int group = static_cast<int>(threadIdx.x) / kLanes, lane = static_cast<int>(threadIdx.x) % kLanes;
-  // the beginning of the tile is part 1 of this CTA, what follows is part 0 of the next ones
-  const auto part = [&](int i) { return parts + (2ll * (cta + i) + (i == 0 ? 1 : 0)) * part_floats<kRows, kD>(); };
-  for (int first = 0; first < rows * kVecs; first += kLanes) {
-    const int i = first + lane;
-    const bool live = i < rows * kVecs;
-    const int r = live ? i / kVecs : 0, d = i % kVecs;
-    float top = kMinusInf, sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c0 = group; c0 < count; c0 += kJoinGroups * kAhead) {
-      float m[kAhead], l[kAhead];
-      float4 v[kAhead];
+  const Split mine = splits[cta];
+#pragma unroll 1
+  for (int role = 0; role < 2; ++role) {  // the tile that this CTA continued, the tile that it began
+    const int first = role == 0 ? mine.first_cta : (mine.last_cta >= 0 ? cta : -1);
+    if (first < 0) continue;
+    const Split sp = role == 0 ? splits[first] : mine;
+    const int count = sp.last_cta - first + 1;
+    // the beginning of the tile is part 1 of its CTA, what follows is part 0 of the next ones
+    const auto part = [&](int i) { return parts + (2ll * (first + i) + (i == 0 ? 1 : 0)) * part_floats<kRows, kD>(); };
+    const int vecs = sp.rows * kVecs;  // of the tile; this block's:
+    const int begin = static_cast<int>(static_cast<long long>(vecs) * (cta - first) / count);
+    const int end = static_cast<int>(static_cast<long long>(vecs) * (cta - first + 1) / count);
+    for (int at = begin; at < end; at += kJoinThreads) {
+      const int n = min(end - at, kJoinThreads);
+      const int groups = min(min(kJoinThreads / n, kGroups), count);
+      const int group = static_cast<int>(threadIdx.x) / n, vec = at + static_cast<int>(threadIdx.x) % n;
+      const int r = vec / kVecs, d = vec % kVecs;
+      RunningSum run = {kMinusInf, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+      if (group < groups) {
+        for (int c0 = group; c0 < count; c0 += groups * kAhead) {
+          float2 ml[kAhead];
+          float4 v[kAhead];
 #pragma unroll
-      for (int x = 0; x < kAhead; ++x) {
-        const int c = c0 + x * kJoinGroups;
-        m[x] = kMinusInf;
-        if (c < count && live) {
-          const float* at = part(c);
-          m[x] = at[kRows * kD + 2 * r];
-          l[x] = at[kRows * kD + 2 * r + 1];
-          v[x] = reinterpret_cast<const float4*>(at)[r * kVecs + d];
-        } else {
-          l[x] = 0.0f;
-          v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int x = 0; x < kAhead; ++x) {
+            const int c = c0 + x * groups;
+            ml[x] = make_float2(kMinusInf, 0.0f);
+            v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c < count) {
+              ml[x] = *reinterpret_cast<const float2*>(part(c) + kRows * kD + 2 * r);
+              v[x] = reinterpret_cast<const float4*>(part(c))[vec];
+            }
+          }
+          float ref = run.top;
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) ref = fmaxf(ref, ml[x].x);
+          run.move_to(ref);
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) run.add(ml[x].x, ml[x].y, v[x]);
         }
       }
-      float ref = top;
-#pragma unroll
-      for (int x = 0; x < kAhead; ++x) ref = fmaxf(ref, m[x]);
-      const float base = ref == kMinusInf ? 0.0f : ref;
-      const float old = exp2_approx(top - base);
-      top = ref;
-      sum *= old;
-      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-#pragma unroll
-      for (int x = 0; x < kAhead; ++x) {
-        const float f = exp2_approx(m[x] - base);
-        sum = fmaf(l[x], f, sum);
-        acc.x = fmaf(v[x].x, f, acc.x);
-        acc.y = fmaf(v[x].y, f, acc.y);
-        acc.z = fmaf(v[x].z, f, acc.z);
-        acc.w = fmaf(v[x].w, f, acc.w);
+      if (groups > 1) {
+        group_acc[threadIdx.x] = run.acc;
+        group_ml[threadIdx.x] = make_float2(run.top, run.sum);
+        __syncthreads();
       }
-    }
-    __shared__ float tops[kJoinGroups - 1][kLanes];
-    if (group > 0) {
-      sums[group - 1][lane] = acc;
-      weights[group - 1][lane] = sum;
-      tops[group - 1][lane] = top;
-    }
-    __syncthreads();
-    if (group == 0 && live) {
-      float ref = top;
-#pragma unroll
-      for (int x = 0; x < kJoinGroups - 1; ++x) ref = fmaxf(ref, tops[x][lane]);
-      const float base = ref == kMinusInf ? 0.0f : ref;
-      const float old = exp2_approx(top - base);
-      sum *= old;
-      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-#pragma unroll
-      for (int x = 0; x < kJoinGroups - 1; ++x) {
-        const float f = exp2_approx(tops[x][lane] - base);
-        const float4 v = sums[x][lane];
-        sum = fmaf(weights[x][lane], f, sum);
-        acc.x = fmaf(v.x, f, acc.x);
-        acc.y = fmaf(v.y, f, acc.y);
-        acc.z = fmaf(v.z, f, acc.z);
-        acc.w = fmaf(v.w, f, acc.w);
+      if (group == 0) {
+        float ref = run.top;
+        for (int x = 1; x < groups; ++x) ref = fmaxf(ref, group_ml[threadIdx.x + x * n].x);
+        run.move_to(ref);
+        for (int x = 1; x < groups; ++x) {
+          const float2 ml = group_ml[threadIdx.x + x * n];
+          run.add(ml.x, ml.y, group_acc[threadIdx.x + x * n]);
+        }
+        store_row(p, sp.q_base, sp.kv_head, sp.row0 + r, 4 * d, run.acc, run.top, run.sum);
       }
-      store_row(p, cur.s, cur.kv_head, cur.row0 + r, 4 * d, acc, ref, sum);
+      if (groups > 1) __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -945,7 +994,7 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<kD, kNT, S::kUnit>, p);
+  return cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<kD, kNT>, p);
 }
 
 template <int kD, int kSub>
