@@ -370,6 +370,12 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
   constexpr int kRowVecs = kD / 16;         // 16-byte vectors of a row
   constexpr int kCopyRows = 32 / kRowVecs;  // rows that one copy instruction of the warp covers
   const int copy_row = lane / kRowVecs, copy_vec = lane % kRowVecs;
+  constexpr int kPlaces = 8 / kCopyRows > 0 ? 8 / kCopyRows : 1;  // the placement repeats after 8 rows
+  uint32_t copy_at[kPlaces];
+#pragma unroll
+  for (int i = 0; i < kPlaces; ++i) copy_at[i] = place<kD, kChunk>(i * kCopyRows + copy_row, copy_vec);
+  constexpr int k8Rows = 8 * (kD == 64 ? 64 : 128);  // bytes from a row to the one 8 further
+  const bool dense = p.k_row == kD && p.v_row == kD;
   // operand rows: K tokens g and g + 8 of 16; V tokens 2t, 2t + 1 and those + 8 (the placement repeats after 8 rows)
   int k_at[kD / 64], v_at[2][S::kVH];
 #pragma unroll
@@ -381,7 +387,6 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
       const int row = token_of<kD>(2 * t + i);
       v_at[i][h] = S::kTileBytes + (kD == 64 ? place<kD, kChunk>(row, g >> 1) + 8 * (g & 1) : place<kD, kChunk>(row, 8 * h + g));
     }
-  constexpr int k8Rows = 8 * (kD == 64 ? 64 : 128);  // bytes from a row to the one 8 further
   __shared__ float join_ml[kWarps][S::kRows][2];
   __shared__ __align__(8) float row_scale[S::kRows];  // of a query row: what its scores are multiplied by, in units of log2
   __shared__ __align__(8) int row_end[S::kRows];      // the tokens it sees: [0, end)
@@ -402,30 +407,32 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
         char* const at = ring + stage * S::kStageBytes;
         const uint32_t base = smem_addr(at);
         const int mine = next_page >= 0 && next_page < p.num_pages ? next_page : -1;
+        const bool whole_chunk = token0 + kChunk <= ahead.max_end && __all_sync(0xffffffffu, mine >= 0 || lane >= S::kSubs);
+        const auto copy_chunk = [&](auto whole, long long k_step, long long v_step) {  // steps of kCopyRows rows
 #pragma unroll
-        for (int sub = 0; sub < S::kSubs; ++sub) {
-          const int page = __shfl_sync(0xffffffffu, mine, sub);
-          const long long at_page = max(page, 0);
-          const int row0 = ((token0 + sub * kSub) & (p.page_size - 1)) + copy_row;
-          const uint8_t* k = p.k_cache + at_page * p.k_page + ahead.kv_head * p.k_head + row0 * p.k_row + 16 * copy_vec;
-          const uint8_t* v = p.v_cache + at_page * p.v_page + ahead.kv_head * p.v_head + row0 * p.v_row + 16 * copy_vec;
-          const int left = page < 0 ? 0 : ahead.max_end - token0 - sub * kSub;  // tokens of the part that there are
-          if (left >= kSub) {
+          for (int sub = 0; sub < S::kSubs; ++sub) {
+            const int page = __shfl_sync(0xffffffffu, mine, sub);
+            const long long at_page = whole.value ? page : max(page, 0);
+            const int row0 = ((token0 + sub * kSub) & (p.page_size - 1)) + copy_row;
+            const uint8_t* k = p.k_cache + at_page * p.k_page + ahead.kv_head * p.k_head + row0 * p.k_row + 16 * copy_vec;
+            const uint8_t* v = p.v_cache + at_page * p.v_page + ahead.kv_head * p.v_head + row0 * p.v_row + 16 * copy_vec;
+            const int left = page < 0 ? 0 : ahead.max_end - token0 - sub * kSub;  // tokens of the part that there are
 #pragma unroll
-            for (int i = 0; i < kSub; i += kCopyRows) {
-              const uint32_t to = base + place<kD, kChunk>(sub * kSub + i + copy_row, copy_vec);
-              copy_async<16>(to, k + i * p.k_row);
-              copy_async<16>(to + S::kTileBytes, v + i * p.v_row);
-            }
-          } else {  // zeros in place of the others: zero times NaN is NaN
-#pragma unroll
-            for (int i = 0; i < kSub; i += kCopyRows) {
-              const uint32_t to = base + place<kD, kChunk>(sub * kSub + i + copy_row, copy_vec);
-              const bool take = i + copy_row < left;
-              copy_async<16, false>(to, take ? k + i * p.k_row : p.k_cache, take);
-              copy_async<16, false>(to + S::kTileBytes, take ? v + i * p.v_row : p.v_cache, take);
+            for (int n = 0; n < kSub / kCopyRows; ++n) {
+              const int row = sub * kSub + n * kCopyRows;
+              const uint32_t to = base + copy_at[n % kPlaces] + row / 8 * k8Rows;
+              const bool take = whole.value || n * kCopyRows + copy_row < left;
+              copy_async<16, whole.value>(to, take ? k + n * k_step : p.k_cache, take);
+              copy_async<16, whole.value>(to + S::kTileBytes, take ? v + n * v_step : p.v_cache, take);
             }
           }
+        };
+        if (!whole_chunk) {  // zeros in place of the others: zero times NaN is NaN
+          copy_chunk(std::false_type{}, kCopyRows * p.k_row, kCopyRows * p.v_row);
+        } else if (dense) {  // offsets that are known
+          copy_chunk(std::true_type{}, kCopyRows * kD, kCopyRows * kD);
+        } else {
+          copy_chunk(std::true_type{}, kCopyRows * p.k_row, kCopyRows * p.v_row);
         }
         const int page = __shfl_sync(0xffffffffu, mine, lane >> 1);
         if (lane < 2 * S::kSubs) {
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
       for (int i = 0; i < S::kOT; ++i)
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) o[h][i][nt][0] = o[h][i][nt][1] = o[h][i][nt][2] = o[h][i][nt][3] = 0.0f;
-    float v_unit = 1.0f, v_top = 0.0f;  // unit of o, largest unit so far
+    float v_unit = 1.0f, v_top = 1.0f;  // unit of o, the largest so far
     float m[kNT][2], l[kNT][2];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
@@ -544,42 +551,52 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
           qf[nt][0] = lo.x, qf[nt][1] = lo.y, qf[nt][2] = lo.z, qf[nt][3] = lo.w;
           qf[nt][4] = hi.x, qf[nt][5] = hi.y, qf[nt][6] = hi.z, qf[nt][7] = hi.w;
         }
+        uint32_t w[S::kMT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < S::kMT; ++mt) {
-          const uint4 ka = *reinterpret_cast<const uint4*>(base + k_at[j] + 2 * mt * k8Rows);
-          const uint4 kb = *reinterpret_cast<const uint4*>(base + k_at[j] + (2 * mt + 1) * k8Rows);
-          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 2; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(base + k_at[j] + (2 * mt + i) * k8Rows);
+            w[mt][i][0] = v.x, w[mt][i][1] = v.y, w[mt][i][2] = v.z, w[mt][i][3] = v.w;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // neighbouring products do not wait for one another's sums
+#pragma unroll
+          for (int mt = 0; mt < S::kMT; ++mt) {
             uint32_t a0, a1, a2, a3;
-            halves_of(wa[i], a0, a2);
-            halves_of(wb[i], a1, a3);
+            halves_of(w[mt][0][i], a0, a2);
+            halves_of(w[mt][1][i], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) mma16816(s[mt][nt], a0, a1, a2, a3, qf[nt][2 * i], qf[nt][2 * i + 1]);
           }
-        }
       }
-      // ---- softmax over the tokens, column by column
-      float alpha[kNT][2];
+      // ---- softmax over the tokens, column by column.  m is a reference that is at most kSlack below the largest score so
+      // far: O and l are rescaled only when a score passes it by more, which after a few chunks hardly happens (p is then
+      // at most 2^kSlack, well inside fp16, and its relative rounding is the same).
+      constexpr float kSlack = 8.0f;
       uint32_t pf[S::kMT][kNT][2];
+      // Scores of one page: the factor goes into the exponent's argument (it is not negative, so the largest product is
+      // the largest score).  Scores of several pages, or masked ones, are multiplied first.
+      const bool fold = S::kSubs == 1 && !partial;
+      float2 col[kNT];
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        const float2 col = *reinterpret_cast<const float2*>(&row_scale[8 * nt + 2 * t]);
-        // Scores of one page: the factor goes into the exponent's argument (it is not negative, so the largest product is
-        // the largest score).  Scores of several pages, or masked ones, are multiplied first.
-        float e0 = col.x * k_scale[0], e1 = col.y * k_scale[0];
-        if (S::kSubs > 1 || partial) {
+      for (int nt = 0; nt < kNT; ++nt) col[nt] = *reinterpret_cast<const float2*>(&row_scale[8 * nt + 2 * t]);
+      if (!fold) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
           for (int mt = 0; mt < S::kMT; ++mt) {
-            const float f0 = col.x * k_scale[mt * 16 / kSub], f1 = col.y * k_scale[mt * 16 / kSub];
+            const float f0 = col[nt].x * k_scale[mt * 16 / kSub], f1 = col[nt].y * k_scale[mt * 16 / kSub];
             s[mt][nt][0] *= f0;
             s[mt][nt][1] *= f1;
             s[mt][nt][2] *= f0;
             s[mt][nt][3] *= f1;
           }
-          e0 = e1 = 1.0f;
         }
-        if (partial) {
+      }
+      if (partial) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
           const int2 end = *reinterpret_cast<const int2*>(&row_end[8 * nt + 2 * t]);
 #pragma unroll
           for (int mt = 0; mt < S::kMT; ++mt) {
@@ -590,6 +607,11 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
             if (token + 8 >= end.y) s[mt][nt][3] = kMinusInf;
           }
         }
+      }
+      float top[kNT][2];
+      bool passed = false;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
         float top0 = fmaxf(s[0][nt][0], s[0][nt][2]), top1 = fmaxf(s[0][nt][1], s[0][nt][3]);
 #pragma unroll
         for (int mt = 1; mt < S::kMT; ++mt) {
@@ -601,27 +623,70 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
           top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
           top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
         }
-        top0 = fmaxf(m[nt][0], top0 * e0);
-        top1 = fmaxf(m[nt][1], top1 * e1);
+        col[nt].x = fold ? col[nt].x * k_scale[0] : 1.0f;  // what is left to multiply by
+        col[nt].y = fold ? col[nt].y * k_scale[0] : 1.0f;
+        top[nt][0] = top0 * col[nt].x;
+        top[nt][1] = top1 * col[nt].y;
+        passed = passed || top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
+      }
+      if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            f[c] = 1.0f;
+            if (top[nt][c] > m[nt][c] + kSlack) {
+              f[c] = exp2_approx(m[nt][c] - top[nt][c]);
+              m[nt][c] = top[nt][c];
+              l[nt][c] *= f[c];
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < S::kVH; ++h)
+#pragma unroll
+            for (int i = 0; i < S::kOT; ++i) {
+              o[h][i][nt][0] *= f[0];
+              o[h][i][nt][1] *= f[1];
+              o[h][i][nt][2] *= f[0];
+              o[h][i][nt][3] *= f[1];
+            }
+        }
+      }
+      // V scales: O is kept in units of the chunk's largest one, so that products can be added to it where they are; p is
+      // multiplied by what a page's scale is of that, which stays exact enough in fp16 down to an eighth.  (Scales that
+      // are powers of two are mostly alike.)
+      float v_max = 0.0f;
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) v_max = there[sub] ? fmaxf(v_max, v_scale[sub]) : v_max;
+      bool plain = v_max <= kMaxFloat && v_max >= v_top * 0x1p-80f;
+      float share[S::kSubs];
+      const float inv_unit = S::kSubs > 1 ? 1.0f / v_max : 1.0f;
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) {
+        if (S::kSubs > 1) plain = plain && (!there[sub] || v_scale[sub] >= v_max * 0.125f);
+        share[sub] = S::kSubs > 1 && there[sub] ? v_scale[sub] * inv_unit : 1.0f;
+      }
+#pragma unroll
+      for (int sub = 0; sub < S::kSubs; ++sub) share[sub] = plain ? share[sub] : 1.0f;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        const float e0 = col[nt].x, e1 = col[nt].y;
         // a column without a token so far: any finite reference will do
-        const float ref0 = top0 == kMinusInf ? 0.0f : top0;
-        const float ref1 = top1 == kMinusInf ? 0.0f : top1;
-        alpha[nt][0] = exp2_approx(m[nt][0] - ref0);
-        alpha[nt][1] = exp2_approx(m[nt][1] - ref1);
-        m[nt][0] = top0;
-        m[nt][1] = top1;
-        float sum0 = 0.0f, sum1 = 0.0f;
+        const float ref0 = m[nt][0] == kMinusInf ? 0.0f : m[nt][0], ref1 = m[nt][1] == kMinusInf ? 0.0f : m[nt][1];
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
-          const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
-          const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
-          sum0 += p0 + p2;
-          sum1 += p1 + p3;
+          float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
+          float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          if constexpr (S::kSubs > 1) {
+            const float f = share[mt * 16 / kSub];
+            p0 *= f, p1 *= f, p2 *= f, p3 *= f;
+          }
           pf[mt][nt][0] = transpose8x8(half2_of(p0, p1));
           pf[mt][nt][1] = transpose8x8(half2_of(p2, p3));
         }
-        l[nt][0] = l[nt][0] * alpha[nt][0] + sum0;
-        l[nt][1] = l[nt][1] * alpha[nt][1] + sum1;
       }
       bool strange = false;
       if (partial && cur.min_end < cur.max_end) {
@@ -637,12 +702,12 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
         }
         strange = __any_sync(0xffffffffu, bad);
       }
-      // ---- O^T += V^T P^T over one part of the chunk.  Plain: the products are added to O as they are.  cut: V counts as
-      // zero from token `end` of the chunk on, and the columns that `takes` names get f * product.
+      // ---- O^T += V^T P^T.  Plain: the whole chunk, products added to O as they are.  cut: one part of it, V counts as zero
+      // from token `end` of the chunk on, and the columns that `takes` names get f * product.
       const auto product = [&](auto cut, int sub, int end, float f, auto takes) {
 #pragma unroll
         for (int h = 0; h < S::kVH; ++h) {
-          constexpr int kW = S::kVW, kSteps = kSub / 16;
+          constexpr int kW = S::kVW, kSteps = cut.value ? kSub / 16 : S::kMT;
           uint32_t w[kSteps][4][kW];
 #pragma unroll
           for (int ks = 0; ks < kSteps; ++ks)
@@ -664,79 +729,71 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
                 }
               }
             }
+          float d[kW][2][kNT][4];
+          if constexpr (cut.value) {
 #pragma unroll
-          for (int c = 0; c < kW; ++c) {
+            for (int c = 0; c < kW; ++c)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float(&acc)[kNT][4] = o[h][2 * c + half];
-              float d[kNT][4];
+              for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.0f;
+                for (int e = 0; e < 4; ++e) d[c][0][nt][e] = d[c][1][nt][e] = 0.0f;
+          }
 #pragma unroll
-              for (int ks = 0; ks < kSteps; ++ks) {
+          for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+            for (int c = 0; c < kW; ++c)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
                 const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;  // bytes 2 half, 2 half + 1 of two tokens, interleaved
                 const int mt = sub * kSteps + ks;
                 uint32_t a0, a1, a2, a3;
                 halves_of(__byte_perm(w[ks][0][c], w[ks][1][c], pick), a0, a1);
                 halves_of(__byte_perm(w[ks][2][c], w[ks][3][c], pick), a2, a3);
 #pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) mma16816(cut.value ? d[nt] : acc[nt], a0, a1, a2, a3, pf[mt][nt][0], pf[mt][nt][1]);
+                for (int nt = 0; nt < kNT; ++nt) {
+                  mma16816(cut.value ? d[c][half][nt] : o[h][2 * c + half][nt], a0, a1, a2, a3, pf[mt][nt][0], pf[mt][nt][1]);
+                }
               }
-              if constexpr (cut.value) {
+          if constexpr (cut.value) {
+#pragma unroll
+            for (int c = 0; c < kW; ++c)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
-                    if (takes(nt, e & 1)) acc[nt][e] = fmaf(d[nt][e], f, acc[nt][e]);
+                    if (takes(nt, e & 1)) o[h][2 * c + half][nt][e] = fmaf(d[c][half][nt][e], f, o[h][2 * c + half][nt][e]);
                   }
-              }
-            }
           }
         }
       };
-      // O is kept in units of the V scale of the page that was added last, so that products can be added to it where they
-      // are: O moves to a new unit together with the rescaling that a new maximum asks for, and mostly neither changes.
-      // A scale that is zero, not finite or 2^80 below the largest so far would take O out of fp32's range; such a part
-      // is multiplied on its own and added with its factor.
-      bool rescale = false;  // by alpha
+      if (!strange && plain) {
+        if (v_max != v_unit) {
+          const float ratio = v_unit / v_max;
+          v_unit = v_max;
+          v_top = fmaxf(v_top, v_max);
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) rescale = rescale || alpha[nt][0] != 1.0f || alpha[nt][1] != 1.0f;
-      rescale = __any_sync(0xffffffffu, rescale);
+          for (int h = 0; h < S::kVH; ++h)
 #pragma unroll
-      for (int sub = 0; sub < S::kSubs; ++sub) {
-        if (!there[sub]) continue;
-        const float vs = v_scale[sub];
-        const bool plain = !strange && vs <= kMaxFloat && vs > 0.0f && vs >= v_top * 0x1p-80f;
-        float ratio = 1.0f;
-        if (plain && vs != v_unit) {
-          if (v_top > 0.0f) ratio = __fdividef(v_unit, vs);
-          v_unit = vs;
+            for (int i = 0; i < S::kOT; ++i)
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[h][i][nt][e] *= ratio;
         }
-        if (plain) v_top = fmaxf(v_top, vs);
-        if (rescale || ratio != 1.0f) {
+        product(std::false_type{}, 0, 0, 1.0f, [](int, int) { return true; });
+      } else {
+        // Something that is not finite, or scales too far apart (zero, or 2^80 below the largest so far, would take O out
+        // of fp32's range): every part on its own, added with its factor, once for every place where a column's context
+        // can end in the part or behind it, with V cut there; columns that see nothing of the part take nothing from it.
+        const int lo = min(max(cur.min_end - token0, 0), kChunk), hi = min(cur.max_end - token0, kChunk);
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            const float f0 = rescale ? alpha[nt][0] * ratio : ratio, f1 = rescale ? alpha[nt][1] * ratio : ratio;
-#pragma unroll
-            for (int h = 0; h < S::kVH; ++h)
-#pragma unroll
-              for (int i = 0; i < S::kOT; ++i) {
-                o[h][i][nt][0] *= f0;
-                o[h][i][nt][1] *= f1;
-                o[h][i][nt][2] *= f0;
-                o[h][i][nt][3] *= f1;
-              }
-          }
-          rescale = false;
-        }
-        if (plain) {
-          product(std::false_type{}, sub, 0, 1.0f, [](int, int) { return true; });
-        } else {
-          // once for every place where a column's context can end in this part or behind it, with V cut there; columns
-          // that see nothing of the part take nothing from it
-          const int lo = min(max(cur.min_end - token0, 0), kChunk), hi = min(cur.max_end - token0, kChunk);
+        for (int sub = 0; sub < S::kSubs; ++sub) {
+          if (!there[sub]) continue;
+          const float f = v_scale[sub] / (plain ? v_unit * share[sub] : v_unit);  // p has its share already
           for (int end = max(lo, sub * kSub + 1); end <= hi; ++end) {
-            product(std::true_type{}, sub, end, vs / v_unit, [&](int nt, int c) {
+            product(std::true_type{}, sub, end, f, [&](int nt, int c) {
               return min(row_end[8 * nt + 2 * t + c] - token0, kChunk) == end;
             });
           }
