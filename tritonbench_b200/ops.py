@@ -6,7 +6,6 @@ Mirrors the call the reference backends make,
 (tritonbench/operators/fp8_gemm_rowwise/operator.py:187-217): same argument order and meaning,
 a fresh bf16 [M, N] tensor as the result.
 """
-import contextlib
 from typing import Callable, Dict, Optional, Sequence, Tuple
 
 import torch
@@ -335,13 +334,13 @@ def fp8_gemm(a: torch.Tensor, b: torch.Tensor, scale_a=None, scale_b=None, out_d
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# A decode step makes these calls once per layer with kernels of a few microseconds: the checks below are written for
+# their cost (get_device() is a tenth of comparing torch.device objects, the stream handle a thirtieth of a Stream object).
+def _raw_stream_slow(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _on_device_of(t: torch.Tensor):
-    """Context in which t's device is the current one (a launch on a stream of another device is an error)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream_slow)
 
 
 class _Rotary(torch.autograd.Function):
@@ -349,7 +348,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, table, interleaved, transpose):
         ctx.save_for_backward(positions, table)
         ctx.form = (interleaved, transpose)
-        return _rotary(x, positions, table, interleaved, transpose, None)
+        return rotary(x, positions, table, interleaved, transpose)
 
     @staticmethod
     def backward(ctx, grad):
@@ -360,23 +359,6 @@ class _Rotary(torch.autograd.Function):
         return rotary(grad, positions, table, interleaved, not transpose), None, None, None, None
 
 
-def _rotary(x, positions, table, interleaved, transpose, out):
-    tokens, heads, dim = x.shape
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
-    if tokens == 0 or heads == 0:
-        return out
-    sx, sy = x.stride(), out.stride()
-    with _on_device_of(x):
-        status = _lib.load().b200fp8_rotary(
-            x.data_ptr(), _DTYPES[x.dtype], out.data_ptr(), tokens, heads, dim, sx[0], sx[1], sy[0], sy[1],
-            positions.data_ptr(), positions.dtype == torch.int64, table.data_ptr(), table.shape[0], table.shape[1],
-            interleaved, transpose, _stream(x.device),
-        )
-    _lib.check(status, f"b200fp8_rotary({tokens}x{heads}x{dim}, {x.dtype})")
-    return out
-
-
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interleaved: bool = False,
            transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary positions of x [tokens, heads, dim] (bf16, fp16 or fp32; any token and head stride, so a view of a fused
@@ -385,31 +367,50 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     int64; table float32 [max_positions, rot] from `rotary.rotary_table`; a position outside it gives NaN.
     fp32 arithmetic, one rounding.  out may be x.  transpose=True is the gradient with regard to x; a call on an x that
     requires one is differentiable."""
-    for t, name in ((x, "x"), (positions, "positions"), (table, "table")):
-        _require_cuda(t, name)
-        if t.device != x.device:
-            raise ValueError(f"{name} must be on x's device")
-    if x.dim() != 3 or x.stride(2) != 1:
-        raise ValueError("x must be [tokens, heads, dim] with dim contiguous")
-    if x.dtype not in _DTYPES:
+    device = x.get_device()
+    if device < 0:
+        _require_cuda(x, "x")
+    if positions.get_device() != device or table.get_device() != device:
+        raise ValueError("positions and table must be on x's device")
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise ValueError(f"unsupported dtype {x.dtype}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or not positions.is_contiguous():
+    if x.dim() != 3:
+        raise ValueError("x must be [tokens, heads, dim]")
+    tokens, heads, dim = x.shape
+    x_token, x_head, one = x.stride()
+    if one != 1 and dim > 1:
+        raise ValueError("x must have dim contiguous")
+    wide = positions.dtype is torch.int64
+    if not wide and positions.dtype is not torch.int32 or positions.dim() != 1 or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 vector")
-    if positions.numel() != x.shape[0]:
+    if positions.numel() != tokens:
         raise ValueError("positions must have one entry per token")
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+    if table.dtype is not torch.float32 or table.dim() != 2 or not table.is_contiguous():
         raise ValueError("table must be a contiguous float32 [max_positions, rot]")
-    if not 2 <= table.shape[1] <= x.shape[2] or table.shape[1] % 2:
-        raise ValueError("the table's width must be even and at most dim")
-    interleaved, transpose = bool(interleaved), bool(transpose)
-    if torch.is_grad_enabled() and x.requires_grad:
+    max_pos, rot = table.shape
+    if max_pos < 1 or not 2 <= rot <= dim or rot % 2:
+        raise ValueError("the table needs a row, and an even width of at most dim")
+    if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
         return _Rotary.apply(x, positions, table, interleaved, transpose)
-    if out is not None:
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
-            raise ValueError("out must have x's shape, dtype and device, dim contiguous")
-    return _rotary(x, positions, table, interleaved, transpose, out)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != device or out.stride(2) != 1:
+        raise ValueError("out must have x's shape, dtype and device, dim contiguous")
+    if tokens == 0 or heads == 0:
+        return out
+    if device != torch.cuda.current_device():  # a launch on a stream of another device is an error
+        with torch.cuda.device(device):
+            return rotary(x, positions, table, interleaved, transpose, out)
+    y_token, y_head, _ = out.stride()
+    status = _lib.load().b200fp8_rotary(
+        x.data_ptr(), dtype, out.data_ptr(), tokens, heads, dim, x_token, x_head, y_token, y_head, positions.data_ptr(), wide,
+        table.data_ptr(), max_pos, rot, bool(interleaved), bool(transpose), _raw_stream(device))
+    if status:
+        _lib.check(status, f"b200fp8_rotary({tokens}x{heads}x{dim}, {x.dtype})")
+    return out
 
 
 class Fp8KvCache:
@@ -418,7 +419,7 @@ class Fp8KvCache:
     a value is code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object describes the four tensors
     and keeps them alive; make one with `empty`, or around tensors of your own."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "descriptor")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         for t, name in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
@@ -442,6 +443,7 @@ class Fp8KvCache:
                 raise NotImplementedError("rows of k and v must start on 16-byte boundaries")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
+        self.device = k.get_device()
         self.descriptor = _lib.KV_CACHE.pack(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3],
             *k_scale.stride(), *v_scale.stride(), pages, heads, size, dim)
@@ -455,39 +457,32 @@ class Fp8KvCache:
         return cls(k, v, ks, vs)
 
 
-def _check_rows(x: torch.Tensor, name: str, cache: Fp8KvCache) -> None:
-    if x.device != cache.k.device:
-        raise ValueError(f"{name} must be on the cache's device")
-    if x.dim() != 3 or x.shape[2] != cache.head_dim or x.stride(2) != 1:
-        raise ValueError(f"{name} must be [tokens, heads, {cache.head_dim}] with head_dim contiguous")
-    if x.dtype != torch.bfloat16 and x.dtype != torch.float16:
-        raise ValueError(f"{name} must be bfloat16 or float16")
-
-
 def _pack_batch(tokens: int, cache: Fp8KvCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                 cu_seqlens: Optional[torch.Tensor]) -> bytes:
-    device = cache.k.device
-    if block_table.device != device or seq_lens.device != device:
+    device = cache.device
+    if block_table.get_device() != device or seq_lens.get_device() != device:
         raise ValueError("block_table and seq_lens must be on the cache's device")
-    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+    if seq_lens.dtype is not torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32 vector")
-    batch = seq_lens.shape[0]
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 [batch, pages]")
-    width = block_table.shape[1]
-    if width > 1 and block_table.stride(1) != 1:
+    batch, width = block_table.shape
+    pitch, one = block_table.stride()
+    if batch != seq_lens.shape[0]:
+        raise ValueError("block_table and seq_lens must have one row and one entry per sequence")
+    if one != 1 and width > 1:
         raise ValueError("block_table must have its pages contiguous")
+    cu = 0
     if cu_seqlens is None:
         if tokens != batch:
             raise ValueError(f"{tokens} tokens for {batch} sequences: pass cu_seqlens unless every sequence has one")
-        cu = 0
     else:
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] != batch + 1:
+        if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] != batch + 1:
             raise ValueError("cu_seqlens must be a contiguous int32 vector with batch + 1 entries")
-        if cu_seqlens.device != device:
+        if cu_seqlens.get_device() != device:
             raise ValueError("cu_seqlens must be on the cache's device")
         cu = cu_seqlens.data_ptr()
-    return _lib.KV_BATCH.pack(block_table.data_ptr(), seq_lens.data_ptr(), cu, max(block_table.stride(0), width), width, batch, tokens)
+    return _lib.KV_BATCH.pack(block_table.data_ptr(), seq_lens.data_ptr(), cu, pitch if pitch > width else width, width, batch, tokens)
 
 
 def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tensor,
@@ -510,44 +505,58 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     behind cu_seqlens[-1]; in a fresh result they are zero.  Two sequences must not append to the same page."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
-    _check_rows(k, "k", cache)
-    _check_rows(v, "v", cache)
-    if k.shape != v.shape or k.shape[1] != cache.kv_heads or k.dtype != v.dtype:
-        raise ValueError(f"k and v must be [tokens, {cache.kv_heads}, {cache.head_dim}] of one dtype")
-    tokens, heads = k.shape[0], cache.kv_heads
-    sk, sv = k.stride(), v.stride()
-    sq = so = (0, 0)
-    fill = 0
-    q_ptr = qo_ptr = None
+    device, heads, dim = cache.device, cache.kv_heads, cache.head_dim
+    dtype = k.dtype
+    if k.get_device() != device or v.get_device() != device:
+        raise ValueError("k and v must be on the cache's device")
+    if k.dim() != 3 or k.shape[1] != heads or k.shape[2] != dim or v.shape != k.shape:
+        raise ValueError(f"k and v must be [tokens, {heads}, {dim}]")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16 or v.dtype is not dtype:
+        raise ValueError("k and v must be bfloat16 or float16, both the same")
+    tokens = k.shape[0]
+    k_token, k_head, k_one = k.stride()
+    v_token, v_head, v_one = v.stride()
+    if k_one != 1 or v_one != 1:
+        raise ValueError("k and v must have head_dim contiguous")
+    q_token = q_head = o_token = o_head = fill = 0
+    q_ptr = o_ptr = table_ptr = None
     if q is not None:
-        _check_rows(q, "q", cache)
+        if q.get_device() != device or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim or q.dtype is not dtype:
+            raise ValueError("q must be [tokens, heads, head_dim] with k's tokens, head_dim, dtype and device")
         heads = q.shape[1]
-        if q.shape[0] != tokens or q.dtype != k.dtype or heads < 1 or heads % cache.kv_heads:
-            raise ValueError("q must have k's tokens and dtype, and a multiple of its heads")
+        if heads < 1 or heads % cache.kv_heads:
+            raise ValueError(f"{heads} query heads cannot share {cache.kv_heads} kv heads")
+        q_token, q_head, q_one = q.stride()
+        if q_one != 1:
+            raise ValueError("q must have head_dim contiguous")
         if q_out is None:
-            q_out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-            fill = 1
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or q_out.stride(2) != 1:
-            raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
-        sq, so, q_ptr, qo_ptr = q.stride(), q_out.stride(), q.data_ptr(), q_out.data_ptr()
+            q_out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
+            o_token, o_head, fill = heads * dim, dim, 1
+        else:
+            if q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != device or q_out.stride(2) != 1:
+                raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
+            o_token, o_head, _ = q_out.stride()
+        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
     max_pos = rot = 0
-    table_ptr = None
     if table is not None:
-        if table.device != k.device or table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+        if table.get_device() != device or table.dtype is not torch.float32 or table.dim() != 2 or not table.is_contiguous():
             raise ValueError("table must be a contiguous float32 [max_positions, rot] on the cache's device")
         max_pos, rot = table.shape
-        if not 2 <= rot <= cache.head_dim or rot % 2:
-            raise ValueError("the table's width must be even and at most head_dim")
+        if max_pos < 1 or not 2 <= rot <= dim or rot % 2:
+            raise ValueError("the table needs a row, and an even width of at most head_dim")
         table_ptr = table.data_ptr()
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
-    with _on_device_of(k):
-        status = _lib.load().b200fp8_kv_append(
-            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, _DTYPES[k.dtype], heads, sq[0], sq[1], sk[0], sk[1], sv[0], sv[1],
-            so[0], so[1], cache.descriptor, rows, table_ptr, max_pos, rot, bool(interleaved), fill, _stream(k.device))
+    args = (q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, _DTYPES[dtype], heads, q_token, q_head, k_token, k_head, v_token, v_head,
+            o_token, o_head, cache.descriptor, rows, table_ptr, max_pos, rot, bool(interleaved), fill, _raw_stream(device))
+    if device == torch.cuda.current_device():
+        status = _lib.load().b200fp8_kv_append(*args)
+    else:
+        with torch.cuda.device(device):
+            status = _lib.load().b200fp8_kv_append(*args)
     if status:
-        _lib.check(status, f"b200fp8_kv_append(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={cache.head_dim})")
+        _lib.check(status, f"b200fp8_kv_append(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={dim})")
     return q_out
 
 
@@ -567,28 +576,41 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     not depend on timing.  The workspace is allocated per call, so captured graphs and streams never share one."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
-    _check_rows(q, "q", cache)
+    device = cache.device
+    dtype = q.dtype
+    if q.get_device() != device:
+        raise ValueError("q must be on the cache's device")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError(f"q must be [tokens, heads, {cache.head_dim}]")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError("q must be bfloat16 or float16")
     tokens, heads, dim = q.shape
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads cannot share {cache.kv_heads} kv heads")
+    q_token, q_head, one = q.stride()
+    if one != 1:
+        raise ValueError("q must have head_dim contiguous")
     fill = 0
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-        fill = 1
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
-        raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+        out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
+        o_token, o_head, fill = heads * dim, dim, 1
+    else:
+        if out.shape != q.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
+            raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+        o_token, o_head, _ = out.stride()
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
     if tokens:
+        if device != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return fp8_kv_attention(q, cache, block_table, seq_lens, cu_seqlens, softmax_scale, None if fill else out, return_lse)
         lib = _lib.load()
-        sq, so = q.stride(), out.stride()
-        with _on_device_of(q):
-            nbytes = lib.b200fp8_kv_attention_workspace_bytes(cache.descriptor, rows, heads)
-            ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
-            status = lib.b200fp8_kv_attention(
-                q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), _DTYPES[q.dtype], heads, sq[0], sq[1],
-                so[0], so[1], cache.descriptor, rows, dim ** -0.5 if softmax_scale is None else softmax_scale, fill,
-                ws.data_ptr(), ws.numel(), _stream(q.device))
+        nbytes = lib.b200fp8_kv_attention_workspace_bytes(cache.descriptor, rows, heads)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        status = lib.b200fp8_kv_attention(
+            q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), _DTYPES[dtype], heads, q_token, q_head,
+            o_token, o_head, cache.descriptor, rows, dim ** -0.5 if softmax_scale is None else softmax_scale, fill,
+            ws.data_ptr(), nbytes, _raw_stream(device))
         if status:
             _lib.check(status, f"b200fp8_kv_attention(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={dim})")
     return (out, lse) if return_lse else out
