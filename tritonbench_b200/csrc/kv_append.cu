@@ -97,9 +97,7 @@ __device__ __forceinline__ SlotAt slot_at(int slot, int rot) {
   return {slot * 2 * kN, slot * 2 * kN + kN, false};  // rot is a multiple of a slot
 }
 
-template <bool kInterleaved>
-__device__ __forceinline__ void turn(const KvAppendParams& p, long long pos, int slot, float (&a)[kN], float (&b)[kN]) {
-  float c[kN], s[kN];
+__device__ __forceinline__ void table_row(const KvAppendParams& p, long long pos, int slot, float (&c)[kN], float (&s)[kN]) {
   if (pos < p.max_pos) {
     const float* row = p.table + pos * p.rot + slot * kN;
     load_table<kN>(row, c);
@@ -108,11 +106,17 @@ __device__ __forceinline__ void turn(const KvAppendParams& p, long long pos, int
 #pragma unroll
     for (int i = 0; i < kN; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
   }
+}
+
+template <bool kInterleaved>
+__device__ __forceinline__ void turn(const KvAppendParams& p, long long pos, int slot, float (&a)[kN], float (&b)[kN]) {
+  float c[kN], s[kN];
+  table_row(p, pos, slot, c, s);
   rotate_slot<kN, kInterleaved>(a, b, c, s);
 }
 
 // One page, one kv head, k or v.  kGroup threads: a warp or the block.
-template <typename T, bool kInterleaved, int kGroup>
+template <typename T, bool kInterleaved, int kGroup, int kHold>
 __device__ __forceinline__ void append_page(const KvAppendParams& p, long long work) {
   const int in_group = static_cast<int>(threadIdx.x) % kGroup;
   const int which = static_cast<int>(work & 1);
@@ -162,6 +166,7 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   const int items = rows * slots;
   const float old_scale = held > 0 ? *scale_at : 0.0f;
 
+  // the first kHold slots of a thread stay in registers, rotated; what is beyond them is read and rotated twice
   const auto load = [&](int item, float (&a)[kN], float (&c)[kN], SlotAt& at) {
     const int row = item / slots, slot = item - row * slots;
     at = slot_at<kInterleaved>(slot, rot);
@@ -173,14 +178,33 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
     if (at.turns) turn<kInterleaved>(p, from + row, slot, a, c);
     return row;
   };
+  const auto store = [&](int row, const SlotAt& at, const float (&a)[kN], const float (&c)[kN], float inv) {
+    uint8_t* r = codes + (held + row) * code_row;
+    *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv);
+    *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv);
+  };
 
   float amax = 0.0f;
-  for (int item = in_group; item < items; item += kGroup) {
+  float ka[kHold][kN], kb[kHold][kN];
+  SlotAt kat[kHold];
+  int krow[kHold];
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    if (in_group + i * kGroup < items) krow[i] = load(in_group + i * kGroup, ka[i], kb[i], kat[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    if (in_group + i * kGroup < items) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(finite_abs(ka[i][e]), finite_abs(kb[i][e])));
+    }
+  }
+  for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
     float a[kN], c[kN];
     SlotAt at;
     load(item, a, c, at);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) amax = fmaxf(amax, fmaxf(finite_abs(a[i]), finite_abs(c[i])));
+    for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(finite_abs(a[e]), finite_abs(c[e])));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -212,50 +236,52 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
     }
   }
   if (in_group == 0) *scale_at = scale;
-  for (int item = in_group; item < items; item += kGroup) {
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    if (in_group + i * kGroup < items) store(krow[i], kat[i], ka[i], kb[i], inv);
+  }
+  for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
     float a[kN], c[kN];
     SlotAt at;
     const int row = load(item, a, c, at);
-    uint8_t* r = codes + (held + row) * code_row;
-    *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv);
-    *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv);
+    store(row, at, a, c, inv);
   }
 }
 
-// kItems slots of q a thread; the positions of the block's tokens are looked up once, in shared memory
-constexpr int kItems = 2;
-constexpr int kMaxTokens = kThreads * kItems / 4 + 1;  // a head has at least four slots
+// q: a thread has one slot of kHeads neighbouring heads of a token, as in rotary.cu; the positions of the block's tokens
+// are looked up once, in shared memory, while q is on its way.
+constexpr int kMaxTokens = kThreads / 4 + 1;  // a head has at least four slots
 
-template <typename T, bool kInterleaved>
+template <typename T, bool kInterleaved, int kHeads>
 __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long block) {
   __shared__ long long positions[kMaxTokens];
   const int slots = p.dim / (2 * kN);
-  const unsigned per_token = static_cast<unsigned>(p.heads) * static_cast<unsigned>(slots);
-  const long long first = block * (kThreads * kItems);
+  const unsigned per_token = static_cast<unsigned>((p.heads + kHeads - 1) / kHeads) * static_cast<unsigned>(slots);
+  const long long first = block * kThreads;
   const long long items = static_cast<long long>(p.tokens) * per_token;
-  const long long token0 = first / per_token;
-  const long long in_token0 = first - token0 * per_token;
-  long long token1 = (first + kThreads * kItems - 1) / per_token;
-  if (token1 >= p.tokens) token1 = p.tokens - 1;
-  uint4 ra[kItems], rb[kItems];
-  int local[kItems], head[kItems], slot[kItems];
+  const long long token0 = items <= 0xffffffffll ? static_cast<unsigned>(first) / per_token : first / per_token;
+  const unsigned at = static_cast<unsigned>(first - token0 * per_token) + threadIdx.x;
+  const int local = static_cast<int>(at / per_token);
+  const unsigned in_token = at - local * per_token;
+  const int group = static_cast<int>(in_token / static_cast<unsigned>(slots));
+  const int slot = static_cast<int>(in_token - group * static_cast<unsigned>(slots));
+  const int head0 = group * kHeads;
+  const bool live = first + threadIdx.x < items;
+  const SlotAt e = slot_at<kInterleaved>(slot, p.rot);
+  uint4 ra[kHeads], rb[kHeads];
+  if (live) {
+    const T* x = static_cast<const T*>(p.q) + (token0 + local) * p.q_token + head0 * p.q_head;
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {  // on their way while the positions are looked up
-    const unsigned at = static_cast<unsigned>(in_token0) + threadIdx.x + j * kThreads;
-    local[j] = static_cast<int>(at / per_token);
-    const unsigned in_token = at - local[j] * per_token;
-    head[j] = static_cast<int>(in_token / static_cast<unsigned>(slots));
-    slot[j] = static_cast<int>(in_token - head[j] * static_cast<unsigned>(slots));
-    if (first + threadIdx.x + j * kThreads < items) {
-      const T* x = static_cast<const T*>(p.q) + (token0 + local[j]) * p.q_token + head[j] * p.q_head;
-      const SlotAt e = slot_at<kInterleaved>(slot[j], p.rot);
-      ra[j] = *reinterpret_cast<const uint4*>(x + e.a);
-      rb[j] = *reinterpret_cast<const uint4*>(x + e.b);
+    for (int h = 0; h < kHeads; ++h) {
+      if (head0 + h < p.heads) {
+        ra[h] = *reinterpret_cast<const uint4*>(x + h * p.q_head + e.a);
+        rb[h] = *reinterpret_cast<const uint4*>(x + h * p.q_head + e.b);
+      }
     }
   }
-  const int tokens = static_cast<int>(token1 - token0) + 1;
   // all warps look up the block's tokens, one token a warp at a time
-  for (int i = threadIdx.x >> 5; i < tokens; i += kThreads / 32) {
+  const long long last = min(static_cast<long long>(p.tokens) - 1, token0 + (static_cast<unsigned>(first - token0 * per_token) + kThreads - 1) / per_token);
+  for (int i = threadIdx.x >> 5; i <= last - token0; i += kThreads / 32) {
     const long long t = token0 + i;
     long long pos;
     if (p.cu_seqlens == nullptr) {
@@ -270,58 +296,68 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
     if ((threadIdx.x & 31) == 0) positions[i] = pos;
   }
   __syncthreads();
+  if (!live) return;
+  const long long pos = positions[local];
+  if (pos == -2 && !p.fill_rest) return;
+  T* y = static_cast<T*>(p.q_out) + (token0 + local) * p.qo_token + head0 * p.qo_head;
+  float c[kN], s[kN];
+  if (e.turns && pos >= 0) table_row(p, pos, slot, c, s);
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    if (first + threadIdx.x + j * kThreads >= items) continue;
-    const long long pos = positions[local[j]];
-    if (pos == -2 && !p.fill_rest) continue;
-    T* y = static_cast<T*>(p.q_out) + (token0 + local[j]) * p.qo_token + head[j] * p.qo_head;
-    const SlotAt e = slot_at<kInterleaved>(slot[j], p.rot);
-    float a[kN], b[kN];
-    unpack16<T>(ra[j], a);
-    unpack16<T>(rb[j], b);
-    if (pos < 0) {  // not a token of any sequence
-#pragma unroll
-      for (int i = 0; i < kN; ++i) a[i] = b[i] = 0.0f;
-    } else if (e.turns) {
-      turn<kInterleaved>(p, pos, slot[j], a, b);
+  for (int h = 0; h < kHeads; ++h) {
+    if (head0 + h < p.heads) {
+      if (pos < 0) {  // not a token of any sequence
+        ra[h] = rb[h] = make_uint4(0u, 0u, 0u, 0u);
+      } else if (e.turns) {
+        float a[kN], b[kN];
+        unpack16<T>(ra[h], a);
+        unpack16<T>(rb[h], b);
+        rotate_slot<kN, kInterleaved>(a, b, c, s);
+        ra[h] = pack16<T>(a);
+        rb[h] = pack16<T>(b);
+      }
+      *reinterpret_cast<uint4*>(y + h * p.qo_head + e.a) = ra[h];
+      *reinterpret_cast<uint4*>(y + h * p.qo_head + e.b) = rb[h];
     }
-    *reinterpret_cast<uint4*>(y + e.a) = pack16<T>(a);
-    *reinterpret_cast<uint4*>(y + e.b) = pack16<T>(b);
   }
 }
 
-template <typename T, bool kInterleaved, int kGroup>
+template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks) {
   if (blockIdx.x < page_blocks) {
     constexpr int kPerBlock = kThreads / kGroup;
     const long long work = static_cast<long long>(blockIdx.x) * kPerBlock + threadIdx.x / kGroup;
-    if (work < works) append_page<T, kInterleaved, kGroup>(p, work);
+    if (work < works) append_page<T, kInterleaved, kGroup, kHold>(p, work);
   } else {
-    rotate_q<T, kInterleaved>(p, static_cast<long long>(blockIdx.x - page_blocks));
+    rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(blockIdx.x - page_blocks));
   }
 }
 
-template <typename T, bool kInterleaved, int kGroup>
+template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
 cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
   const long long page_slots = p.cu_seqlens == nullptr ? p.batch : (p.tokens >> p.page_shift) + 2ll * p.batch;
   const long long works = page_slots * p.kv_heads * 2;
   const long long page_blocks = (works + kThreads / kGroup - 1) / (kThreads / kGroup);
-  const long long items = p.q == nullptr ? 0 : static_cast<long long>(p.tokens) * p.heads * (p.dim / (2 * kN));
-  const long long q_blocks = (items + kThreads * kItems - 1) / (kThreads * kItems);
+  const long long items = p.q == nullptr ? 0 : static_cast<long long>(p.tokens) * ((p.heads + kHeads - 1) / kHeads) * (p.dim / (2 * kN));
+  const long long q_blocks = (items + kThreads - 1) / kThreads;
   if (page_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (page_blocks + q_blocks == 0) return cudaSuccess;
-  kv_append_kernel<T, kInterleaved, kGroup><<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(
-      p, works, static_cast<unsigned>(page_blocks));
+  kv_append_kernel<T, kInterleaved, kGroup, kHold, kHeads>
+      <<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(p, works, static_cast<unsigned>(page_blocks));
   return cudaGetLastError();
+}
+
+template <typename T, bool kInterleaved>
+cudaError_t launch_i(const KvAppendParams& p, cudaStream_t stream) {
+  // about one token a sequence: a block for every page would leave nearly all of its threads idle
+  if (p.cu_seqlens == nullptr || p.tokens <= 2ll * p.batch) return launch_t<T, kInterleaved, 32, 1, 1>(p, stream);
+  // two slots a thread: a warp for 16 tokens of 64, a block for 64 tokens of 128
+  if (p.page_size * (p.dim / (2 * kN)) <= 64) return launch_t<T, kInterleaved, 32, 2, 4>(p, stream);
+  return launch_t<T, kInterleaved, kThreads, 2, 4>(p, stream);
 }
 
 template <typename T>
 cudaError_t launch_any(const KvAppendParams& p, cudaStream_t stream) {
-  // about one token a sequence: a block for every page would leave nearly all of its threads idle
-  const bool warps = p.cu_seqlens == nullptr || p.tokens <= 2ll * p.batch;
-  if (p.interleaved) return warps ? launch_t<T, true, 32>(p, stream) : launch_t<T, true, kThreads>(p, stream);
-  return warps ? launch_t<T, false, 32>(p, stream) : launch_t<T, false, kThreads>(p, stream);
+  return p.interleaved ? launch_i<T, true>(p, stream) : launch_i<T, false>(p, stream);
 }
 
 }  // namespace

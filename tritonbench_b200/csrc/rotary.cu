@@ -1,11 +1,12 @@
 // Rotary positions of x [tokens, heads, dim] (any token and head pitch, dim contiguous), out of place or in place, and
 // the transposed rotation, which is the gradient with regard to x (sin -> -sin).
 //
-// Bound by HBM: x in, y out, one table row per token.  One thread owns one slot of one head (two 16-byte vectors of
-// x, see rotary.cuh), reads both before it writes either - so in place needs nothing more - and ends.  The two loads
-// of a thread do not wait for the position and the table row (they are issued first), and 40 to 64 KB of x per SM are
-// on their way at full occupancy, which covers HBM latency without a loop or a ring.  The table row of a token is
-// read once per head from L1: twice the bytes of x, but L1 has ten times the bandwidth that HBM leaves an SM.
+// Bound by HBM: x in, y out, one table row per token.  A thread owns one slot (two 16-byte vectors, see rotary.cuh) of
+// kHeads neighbouring heads of a token: it reads all of them before it writes any - so in place needs nothing more -
+// with 2 * kHeads loads in flight that do not wait for the position and the table row, and takes its cosines and sines
+// into registers once for all its heads (once per head they are twice the bytes of x, out of L1, and cost 15 %).
+#include <type_traits>
+
 #include "kernels.h"
 #include "rotary.cuh"
 
@@ -13,15 +14,17 @@ namespace b200fp8 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr long long kManyThreads = 148ll * 2048;  // one wave of one slot a thread
 
 // kN: pairs of a slot (16 bytes of T each; 1: any alignment and any even rot).  Slots [0, rot / 2 / kN) of a head are
-// rotated, the ones behind them copy kN elements each of [rot, dim).
-template <typename T, int kN, bool kInterleaved>
+// rotated, the ones behind them copy 2 * kN elements each of [rot, dim).
+template <typename T, int kN, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
+  using V = typename std::conditional<kN == 1, T, uint4>::type;
   const int half = p.rot / 2;
   const int turning = half / kN;
-  const int slots = turning + (p.copy_rest ? (p.dim - p.rot) / kN : 0);
-  const unsigned per_token = static_cast<unsigned>(p.heads) * static_cast<unsigned>(slots);
+  const int slots = turning + (p.copy_rest ? (p.dim - p.rot + 2 * kN - 1) / (2 * kN) : 0);
+  const unsigned per_token = static_cast<unsigned>((p.heads + kHeads - 1) / kHeads) * static_cast<unsigned>(slots);
   const unsigned long long item = static_cast<unsigned long long>(blockIdx.x) * kThreads + threadIdx.x;
   const unsigned long long items = static_cast<unsigned long long>(p.tokens) * per_token;
   if (item >= items) return;
@@ -35,31 +38,40 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     token = static_cast<long long>(item / per_token);
     in_token = static_cast<unsigned>(item - static_cast<unsigned long long>(token) * per_token);
   }
-  const unsigned head = in_token / static_cast<unsigned>(slots);
-  const int slot = static_cast<int>(in_token - head * static_cast<unsigned>(slots));
-  const T* x = static_cast<const T*>(p.x) + token * p.x_token + static_cast<long long>(head) * p.x_head;
-  T* y = static_cast<T*>(p.y) + token * p.y_token + static_cast<long long>(head) * p.y_head;
-  if (slot >= turning) {  // beyond the rotated part
-    const int at = p.rot + (slot - turning) * kN;
-    if constexpr (kN == 1) {
-      y[at] = x[at];
-    } else {
-      *reinterpret_cast<uint4*>(y + at) = *reinterpret_cast<const uint4*>(x + at);
+  const unsigned group = in_token / static_cast<unsigned>(slots);
+  const int slot = static_cast<int>(in_token - group * static_cast<unsigned>(slots));
+  const int head0 = static_cast<int>(group) * kHeads;
+  const bool turns = slot < turning;
+  int at_a, at_b;
+  if (turns) {
+    at_a = kInterleaved ? 2 * slot * kN : slot * kN;
+    at_b = kInterleaved ? at_a + kN : at_a + half;
+  } else {
+    at_a = p.rot + (slot - turning) * 2 * kN;
+    at_b = at_a + kN;
+  }
+  const bool has_b = at_b < p.dim;
+  const T* x = static_cast<const T*>(p.x) + token * p.x_token + head0 * p.x_head;
+  V ra[kHeads], rb[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (head0 + h < p.heads) {
+      ra[h] = *reinterpret_cast<const V*>(x + h * p.x_head + at_a);
+      if (has_b) rb[h] = *reinterpret_cast<const V*>(x + h * p.x_head + at_b);
+    }
+  }
+  T* y = static_cast<T*>(p.y) + token * p.y_token + head0 * p.y_head;
+  if (!turns) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      if (head0 + h < p.heads) {
+        *reinterpret_cast<V*>(y + h * p.y_head + at_a) = ra[h];
+        if (has_b) *reinterpret_cast<V*>(y + h * p.y_head + at_b) = rb[h];
+      }
     }
     return;
   }
-  const int at_a = kInterleaved ? 2 * slot * kN : slot * kN;
-  const int at_b = kInterleaved ? at_a + kN : at_a + half;
-  float a[kN], b[kN], c[kN], s[kN];
-  if constexpr (kN == 1) {
-    a[0] = to_f32<T>(x[at_a]);
-    b[0] = to_f32<T>(x[at_b]);
-  } else {
-    const uint4 ra = *reinterpret_cast<const uint4*>(x + at_a);
-    const uint4 rb = *reinterpret_cast<const uint4*>(x + at_b);
-    unpack16<T>(ra, a);
-    unpack16<T>(rb, b);
-  }
+  float c[kN], s[kN];
   const long long pos = p.positions_64 ? static_cast<const long long*>(p.positions)[token]
                                        : static_cast<const int*>(p.positions)[token];
   if (pos >= 0 && pos < p.max_pos) {
@@ -74,27 +86,39 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
 #pragma unroll
     for (int i = 0; i < kN; ++i) s[i] = -s[i];
   }
-  rotate_slot<kN, kInterleaved>(a, b, c, s);
-  if constexpr (kN == 1) {
-    y[at_a] = from_f32<T>(a[0]);
-    y[at_b] = from_f32<T>(b[0]);
-  } else {
-    *reinterpret_cast<uint4*>(y + at_a) = pack16<T>(a);
-    *reinterpret_cast<uint4*>(y + at_b) = pack16<T>(b);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (head0 + h < p.heads) {
+      float a[kN], b[kN];
+      if constexpr (kN == 1) {
+        a[0] = to_f32<T>(ra[h]);
+        b[0] = to_f32<T>(rb[h]);
+      } else {
+        unpack16<T>(ra[h], a);
+        unpack16<T>(rb[h], b);
+      }
+      rotate_slot<kN, kInterleaved>(a, b, c, s);
+      if constexpr (kN == 1) {
+        y[h * p.y_head + at_a] = from_f32<T>(a[0]);
+        y[h * p.y_head + at_b] = from_f32<T>(b[0]);
+      } else {
+        *reinterpret_cast<uint4*>(y + h * p.y_head + at_a) = pack16<T>(a);
+        *reinterpret_cast<uint4*>(y + h * p.y_head + at_b) = pack16<T>(b);
+      }
+    }
   }
 }
 
-template <typename T, int kN>
+template <typename T, int kN, int kHeads>
 cudaError_t launch_t(const RotaryParams& p, cudaStream_t stream) {
-  const unsigned long long slots = p.rot / 2 / kN + (p.copy_rest ? (p.dim - p.rot) / kN : 0);
-  const unsigned long long items = static_cast<unsigned long long>(p.tokens) * p.heads * slots;
-  if (items == 0) return cudaSuccess;
+  const unsigned long long slots = p.rot / 2 / kN + (p.copy_rest ? (p.dim - p.rot + 2 * kN - 1) / (2 * kN) : 0);
+  const unsigned long long items = static_cast<unsigned long long>(p.tokens) * ((p.heads + kHeads - 1) / kHeads) * slots;
   const unsigned long long blocks = (items + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
   if (p.interleaved) {
-    rotary_kernel<T, kN, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
+    rotary_kernel<T, kN, true, kHeads><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
   } else {
-    rotary_kernel<T, kN, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
+    rotary_kernel<T, kN, false, kHeads><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
   }
   return cudaGetLastError();
 }
@@ -103,7 +127,11 @@ template <typename T>
 cudaError_t launch_any(const RotaryParams& p, cudaStream_t stream) {
   constexpr int kN = 16 / sizeof(T);
   const bool vector = p.vector_ok && (p.rot / 2) % kN == 0 && p.dim % kN == 0;
-  return vector ? launch_t<T, kN>(p, stream) : launch_t<T, 1>(p, stream);
+  if (!vector) return launch_t<T, 1, 1>(p, stream);
+  // few tokens: more threads rather than more loads a thread
+  const long long threads = static_cast<long long>(p.tokens) * p.heads * (p.dim / (2 * kN));
+  if (threads >= kManyThreads) return launch_t<T, kN, 4>(p, stream);
+  return launch_t<T, kN, 1>(p, stream);
 }
 
 }  // namespace
