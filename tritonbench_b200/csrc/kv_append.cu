@@ -13,10 +13,10 @@
 // as NaN.
 //
 // Bound by HBM for prompts (q in, q out, k and v in at 2 bytes, out at 1), by latency for single tokens.  One launch
-// does it all.  The first blocks own the pages: each group of threads has one (page, kv head, k or v), so that nothing
-// but that group reads or writes the page's scale: no atomics and the same result every time.  The remaining blocks
-// rotate q.  A group is a warp when a sequence brings about one token, else a block; it passes over its rows twice
-// (maximum, then codes), the second time out of L1.
+// does it all.  Some blocks own pages: each group of threads has one (page, kv head, k or v), so that nothing but that
+// group reads or writes the page's scale: no atomics and the same result every time.  The other blocks rotate q.  A
+// group is a warp when a sequence brings about one token or a page is small, else a block; its rows stay in registers
+// between the maximum and the codes.
 #include <cuda_fp8.h>
 
 #include "kernels.h"
@@ -148,37 +148,34 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   const long long from = lo > begin ? lo : begin;
   const long long to = lo + p.page_size < end ? lo + p.page_size : end;
   if (from >= to) return;
-  const int page = p.block_table[b * p.bt_stride + page_no];
-  if (page < 0 || page >= p.num_pages) return;
   const long long token0 = first_token + (from - begin);
   const int rows = static_cast<int>(to - from);
   if (token0 < 0 || token0 + rows > p.tokens) return;  // lengths that do not belong to this q, k, v
   const int held = static_cast<int>(from - lo);
-
+  const int page = p.block_table[b * p.bt_stride + page_no];  // on its way while the rows are read
   const T* x = which ? static_cast<const T*>(p.v) + token0 * p.v_token + head * p.v_head
                      : static_cast<const T*>(p.k) + token0 * p.k_token + head * p.k_head;
   const long long x_token = which ? p.v_token : p.k_token;
-  uint8_t* codes = (which ? p.v_cache : p.k_cache) + page * p.cache_page[which] + head * p.cache_head[which];
-  const long long code_row = p.cache_row[which];
-  float* scale_at = (which ? p.v_scale : p.k_scale) + page * p.scale_page[which] + head * p.scale_head[which];
   const int rot = which ? 0 : p.rot;
   const int slots = p.dim / (2 * kN);
   const int items = rows * slots;
-  const float old_scale = held > 0 ? *scale_at : 0.0f;
 
   // the first kHold slots of a thread stay in registers, rotated; what is beyond them is read and rotated twice
-  const auto load = [&](int item, float (&a)[kN], float (&c)[kN], SlotAt& at) {
+  const auto load = [&](int item, float (&a)[kN], float (&c)[kN]) {
     const int row = item / slots, slot = item - row * slots;
-    at = slot_at<kInterleaved>(slot, rot);
+    const SlotAt at = slot_at<kInterleaved>(slot, rot);
     const T* r = x + row * x_token;
     const uint4 ra = *reinterpret_cast<const uint4*>(r + at.a);
     const uint4 rb = *reinterpret_cast<const uint4*>(r + at.b);
     unpack16<T>(ra, a);
     unpack16<T>(rb, c);
     if (at.turns) turn<kInterleaved>(p, from + row, slot, a, c);
-    return row;
   };
-  const auto store = [&](int row, const SlotAt& at, const float (&a)[kN], const float (&c)[kN], float inv) {
+  uint8_t* codes = nullptr;
+  const long long code_row = p.cache_row[which];
+  const auto store = [&](int item, const float (&a)[kN], const float (&c)[kN], float inv) {
+    const int row = item / slots;
+    const SlotAt at = slot_at<kInterleaved>(item - row * slots, rot);
     uint8_t* r = codes + (held + row) * code_row;
     *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv);
     *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv);
@@ -186,12 +183,14 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
 
   float amax = 0.0f;
   float ka[kHold][kN], kb[kHold][kN];
-  SlotAt kat[kHold];
-  int krow[kHold];
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
-    if (in_group + i * kGroup < items) krow[i] = load(in_group + i * kGroup, ka[i], kb[i], kat[i]);
+    if (in_group + i * kGroup < items) load(in_group + i * kGroup, ka[i], kb[i]);
   }
+  if (page < 0 || page >= p.num_pages) return;
+  codes = (which ? p.v_cache : p.k_cache) + page * p.cache_page[which] + head * p.cache_head[which];
+  float* const scale_at = (which ? p.v_scale : p.k_scale) + page * p.scale_page[which] + head * p.scale_head[which];
+  const float old_scale = held > 0 ? *scale_at : 0.0f;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
     if (in_group + i * kGroup < items) {
@@ -201,8 +200,7 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   }
   for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
     float a[kN], c[kN];
-    SlotAt at;
-    load(item, a, c, at);
+    load(item, a, c);
 #pragma unroll
     for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(finite_abs(a[e]), finite_abs(c[e])));
   }
@@ -238,13 +236,12 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   if (in_group == 0) *scale_at = scale;
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
-    if (in_group + i * kGroup < items) store(krow[i], kat[i], ka[i], kb[i], inv);
+    if (in_group + i * kGroup < items) store(in_group + i * kGroup, ka[i], kb[i], inv);
   }
   for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
     float a[kN], c[kN];
-    SlotAt at;
-    const int row = load(item, a, c, at);
-    store(row, at, a, c, inv);
+    load(item, a, c);
+    store(item, a, c, inv);
   }
 }
 
@@ -322,13 +319,19 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
 }
 
 template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks) {
-  if (blockIdx.x < page_blocks) {
+__global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks,
+                                                                unsigned period) {
+  // Every period-th block owns pages, the others rotate q: the former wait for one load after another, the latter for
+  // bandwidth, so they fill each other's gaps (17438 tokens: 132 us with the page blocks first, 122 us mixed).  With a
+  // token a sequence the pages take longest and go first (period 1; 250 sequences: 6.3 us, mixed 7.2).  Four blocks an SM
+  // (64 registers, a few spilled in the page part) hide more of the waiting than three: 125 us.
+  const unsigned turn = blockIdx.x / period;
+  if (turn < page_blocks && blockIdx.x == turn * period) {
     constexpr int kPerBlock = kThreads / kGroup;
-    const long long work = static_cast<long long>(blockIdx.x) * kPerBlock + threadIdx.x / kGroup;
+    const long long work = static_cast<long long>(turn) * kPerBlock + threadIdx.x / kGroup;
     if (work < works) append_page<T, kInterleaved, kGroup, kHold>(p, work);
   } else {
-    rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(blockIdx.x - page_blocks));
+    rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(blockIdx.x - min(page_blocks, turn + 1)));
   }
 }
 
@@ -342,7 +345,9 @@ cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
   if (page_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (page_blocks + q_blocks == 0) return cudaSuccess;
   kv_append_kernel<T, kInterleaved, kGroup, kHold, kHeads>
-      <<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(p, works, static_cast<unsigned>(page_blocks));
+      <<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(
+          p, works, static_cast<unsigned>(page_blocks),
+          static_cast<unsigned>(kHold > 1 && page_blocks > 0 ? (page_blocks + q_blocks) / page_blocks : 1));
   return cudaGetLastError();
 }
 
