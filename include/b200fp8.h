@@ -253,8 +253,8 @@ int b200fp8_rotary(const void* x, int dtype, void* y, int64_t tokens, int64_t he
 
 /*
  * A paged key/value cache in e4m3.  k, v: codes [num_pages][kv_heads][page_size][head_dim] with byte pitches per page,
- * head and row (multiples of 16, head_dim contiguous); k_scale, v_scale: one fp32 scale per page and head with element
- * pitches; value = code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The descriptor is read during
+ * head and row (multiples of 16, below 2^31, head_dim contiguous; the cache may be larger); k_scale, v_scale: one fp32
+ * scale per page and head with element pitches, not negative; value = code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The descriptor is read during
  * the call; the memory it points to is the caller's.
  */
 typedef struct b200fp8_kv_cache {

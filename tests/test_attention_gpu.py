@@ -133,6 +133,23 @@ def test_rotary_gradient(cuda_device, interleaved):
     _check_rotated(grad, torch.ones_like(x), pos, table, interleaved, transpose=True)
 
 
+@pytest.mark.parametrize("shape", [(1, 3, 64), (5, 1, 64), (1, 1, 64)])
+def test_expanded_inputs(cuda_device, shape):
+    """Tokens or heads with stride zero: the fresh result must not take over such a layout."""
+    from tritonbench_b200 import ops
+
+    x = torch.randn(*shape, device="cuda").bfloat16().expand(5, 3, 64)
+    pos, table = torch.arange(5, device="cuda"), _table(64, 64)
+    want = ops.rotary(x.contiguous(), pos, table)
+    assert torch.equal(ops.rotary(x, pos, table), want)
+    case = Case([40, 3, 17, 64, 9], None, kv=1, group=3, dim=64, page=64)
+    q = x.expand(5, 3, 64)
+    assert torch.equal(ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens),
+                       ops.fp8_kv_attention(q.contiguous(), case.cache, case.block_table, case.seq_lens))
+    _, k, v = _qkv(case)
+    _check_append(case, q, k[:1].expand(5, 1, 64), v[:1].expand(5, 1, 64), table)
+
+
 def test_rotary_edges(cuda_device):
     from tritonbench_b200 import ops
 

@@ -935,6 +935,13 @@ int check_kv(const b200fp8_kv_cache* c, const b200fp8_kv_batch* r, int64_t heads
   if (!aligned16(c->k) || !aligned16(c->v)) return B200FP8_UNSUPPORTED_ALIGNMENT;
   for (int i = 0; i < 3; ++i) {
     if (c->k_pitch[i] % 16 != 0 || c->v_pitch[i] % 16 != 0) return B200FP8_UNSUPPORTED_ALIGNMENT;
+    const int64_t most = i == 2 ? 0x7FFFFFFFll / c->page_size : 0x7FFFFFFFll;  // offsets inside a page fit 32 bits
+    if (c->k_pitch[i] < 0 || c->v_pitch[i] < 0 || c->k_pitch[i] > most || c->v_pitch[i] > most) return B200FP8_TOO_LARGE;
+  }
+  for (int i = 0; i < 2; ++i) {
+    if (c->k_scale_pitch[i] < 0 || c->v_scale_pitch[i] < 0 || c->k_scale_pitch[i] > 0x7FFFFFFFll || c->v_scale_pitch[i] > 0x7FFFFFFFll) {
+      return B200FP8_TOO_LARGE;
+    }
   }
   return B200FP8_OK;
 }
@@ -951,16 +958,16 @@ KvAttentionParams kv_attention_params(const b200fp8_kv_cache& c, const b200fp8_k
   p.v_cache = static_cast<const uint8_t*>(c.v);
   p.k_scale = c.k_scale;
   p.v_scale = c.v_scale;
-  p.k_page = c.k_pitch[0];
-  p.k_head = c.k_pitch[1];
-  p.k_row = c.k_pitch[2];
-  p.v_page = c.v_pitch[0];
-  p.v_head = c.v_pitch[1];
-  p.v_row = c.v_pitch[2];
-  p.ks_page = c.k_scale_pitch[0];
-  p.ks_head = c.k_scale_pitch[1];
-  p.vs_page = c.v_scale_pitch[0];
-  p.vs_head = c.v_scale_pitch[1];
+  p.k_page = static_cast<int>(c.k_pitch[0]);
+  p.k_head = static_cast<int>(c.k_pitch[1]);
+  p.k_row = static_cast<int>(c.k_pitch[2]);
+  p.v_page = static_cast<int>(c.v_pitch[0]);
+  p.v_head = static_cast<int>(c.v_pitch[1]);
+  p.v_row = static_cast<int>(c.v_pitch[2]);
+  p.ks_page = static_cast<int>(c.k_scale_pitch[0]);
+  p.ks_head = static_cast<int>(c.k_scale_pitch[1]);
+  p.vs_page = static_cast<int>(c.v_scale_pitch[0]);
+  p.vs_head = static_cast<int>(c.v_scale_pitch[1]);
   p.block_table = r.block_table;
   p.bt_stride = r.table_pitch;
   p.seq_lens = r.seq_lens;

@@ -336,8 +336,8 @@ struct KvAttentionParams {
   long long q_token, q_head, o_token, o_head;  // elements
   const uint8_t *k_cache, *v_cache;            // as in KvAppendParams
   const float *k_scale, *v_scale;
-  long long k_page, k_head, k_row, v_page, v_head, v_row;  // bytes
-  long long ks_page, ks_head, vs_page, vs_head;            // elements
+  int k_page, k_head, k_row, v_page, v_head, v_row;  // bytes; a page's rows span less than 2^31
+  int ks_page, ks_head, vs_page, vs_head;            // elements
   const int* block_table;
   long long bt_stride;
   const int* seq_lens;

@@ -127,14 +127,12 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionParams& p, int b) {
 // Cost of a tile besides its units, in units: loading the queries, joining the warps and storing what they found takes a
 // block about 2.3 us, a unit takes it 2.0 us (three blocks an SM, the memory busy).  Runs of equal units without it ended
 // between 67 and 98 us (64 sequences of 1 to 8192 tokens), those with eleven tiles last.
-// With 32 rows (three times the join, two blocks an SM) a tile costs 3: 32 requests of 1 to 6 tokens 143 -> 129 us.
-template <int kRows>
-__host__ __device__ constexpr int tile_cost() { return kRows == 32 ? 3 : 1; }
+constexpr int kTileCost = 1;
 
 template <int kRows, int kUnit>
 __device__ __forceinline__ long long cost_of(const KvAttentionParams& p, int b) {
   const Seq s = seq_of<kRows, kUnit>(p, b);
-  return static_cast<long long>(s.row_tiles) * p.kv_heads * (s.units + tile_cost<kRows>());
+  return static_cast<long long>(s.row_tiles) * p.kv_heads * (s.units + kTileCost);
 }
 
 // Equal shares of `total`: CTA c has [begin(c), begin(c + 1)).
@@ -180,7 +178,7 @@ struct Cursor {
   // cost of a tile that is entered.
   __device__ __forceinline__ void advance(const KvAttentionParams& p, long long& left) {
     if (++unit < s.units || left <= 0) return;
-    left -= tile_cost<kRows>();
+    left -= kTileCost;
     if (left <= 0) return;  // the share ends in front of the tile's first unit
     unit = 0;
     if (++tile == s.row_tiles * p.kv_heads) {
@@ -273,7 +271,7 @@ __device__ __forceinline__ void store_row(const KvAttentionParams& p, int q_base
 }
 
 template <int kD, int kNT, int kSub>
-__global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kernel(const KvAttentionParams p) {
+__global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attention_kernel(const KvAttentionParams p) {
   using S = Shape<kD, kNT, kSub>;
   using C = Cursor<S::kRows, S::kUnit>;
   constexpr int kChunk = S::kChunk, kStages = S::kStages;
@@ -346,7 +344,6 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
   }
   __syncthreads();
 
-  constexpr int kTileCost = tile_cost<S::kRows>();
   C cur;
   cur.b = found_b;
   cur.enter_sequence(p);
@@ -408,31 +405,33 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
         const uint32_t base = smem_addr(at);
         const int mine = next_page >= 0 && next_page < p.num_pages ? next_page : -1;
         const bool whole_chunk = token0 + kChunk <= ahead.max_end && __all_sync(0xffffffffu, mine >= 0 || lane >= S::kSubs);
-        const auto copy_chunk = [&](auto whole, long long k_step, long long v_step) {  // steps of kCopyRows rows
+        const uint8_t* const k_head = p.k_cache + static_cast<long long>(ahead.kv_head) * p.k_head;
+        const uint8_t* const v_head = p.v_cache + static_cast<long long>(ahead.kv_head) * p.v_head;
+        const auto copy_chunk = [&](auto whole, int k_row, int v_row) {
 #pragma unroll
           for (int sub = 0; sub < S::kSubs; ++sub) {
             const int page = __shfl_sync(0xffffffffu, mine, sub);
             const long long at_page = whole.value ? page : max(page, 0);
             const int row0 = ((token0 + sub * kSub) & (p.page_size - 1)) + copy_row;
-            const uint8_t* k = p.k_cache + at_page * p.k_page + ahead.kv_head * p.k_head + row0 * p.k_row + 16 * copy_vec;
-            const uint8_t* v = p.v_cache + at_page * p.v_page + ahead.kv_head * p.v_head + row0 * p.v_row + 16 * copy_vec;
+            const uint8_t* k = k_head + at_page * p.k_page + (row0 * k_row + 16 * copy_vec);
+            const uint8_t* v = v_head + at_page * p.v_page + (row0 * v_row + 16 * copy_vec);
             const int left = page < 0 ? 0 : ahead.max_end - token0 - sub * kSub;  // tokens of the part that there are
 #pragma unroll
             for (int n = 0; n < kSub / kCopyRows; ++n) {
               const int row = sub * kSub + n * kCopyRows;
               const uint32_t to = base + copy_at[n % kPlaces] + row / 8 * k8Rows;
               const bool take = whole.value || n * kCopyRows + copy_row < left;
-              copy_async<16, whole.value>(to, take ? k + n * k_step : p.k_cache, take);
-              copy_async<16, whole.value>(to + S::kTileBytes, take ? v + n * v_step : p.v_cache, take);
+              copy_async<16, whole.value>(to, take ? k + n * kCopyRows * k_row : p.k_cache, take);
+              copy_async<16, whole.value>(to + S::kTileBytes, take ? v + n * kCopyRows * v_row : p.v_cache, take);
             }
           }
         };
         if (!whole_chunk) {  // zeros in place of the others: zero times NaN is NaN
-          copy_chunk(std::false_type{}, kCopyRows * p.k_row, kCopyRows * p.v_row);
+          copy_chunk(std::false_type{}, p.k_row, p.v_row);
         } else if (dense) {  // offsets that are known
-          copy_chunk(std::true_type{}, kCopyRows * kD, kCopyRows * kD);
+          copy_chunk(std::true_type{}, kD, kD);
         } else {
-          copy_chunk(std::true_type{}, kCopyRows * p.k_row, kCopyRows * p.v_row);
+          copy_chunk(std::true_type{}, p.k_row, p.v_row);
         }
         const int page = __shfl_sync(0xffffffffu, mine, lane >> 1);
         if (lane < 2 * S::kSubs) {
@@ -440,8 +439,8 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
             *reinterpret_cast<uint32_t*>(at + 2 * S::kTileBytes + 4 * lane) = kNoPage;
           } else {
             copy_async<4>(base + 2 * S::kTileBytes + 4 * lane,
-                          (lane & 1) ? p.v_scale + page * p.vs_page + ahead.kv_head * p.vs_head
-                                     : p.k_scale + page * p.ks_page + ahead.kv_head * p.ks_head);
+                          (lane & 1) ? p.v_scale + static_cast<long long>(page) * p.vs_page + static_cast<long long>(ahead.kv_head) * p.vs_head
+                                     : p.k_scale + static_cast<long long>(page) * p.ks_page + static_cast<long long>(ahead.kv_head) * p.ks_head);
           }
         }
       }
@@ -575,58 +574,53 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
       // at most 2^kSlack, well inside fp16, and its relative rounding is the same).
       constexpr float kSlack = 8.0f;
       uint32_t pf[S::kMT][kNT][2];
-      // Scores of one page: the factor goes into the exponent's argument (it is not negative, so the largest product is
-      // the largest score).  Scores of several pages, or masked ones, are multiplied first.
-      const bool fold = S::kSubs == 1 && !partial;
+      // The factor of a page's scores goes into the exponent's argument (it is not negative, so the largest product is the
+      // largest score); masked scores are multiplied first.
       float2 col[kNT];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) col[nt] = *reinterpret_cast<const float2*>(&row_scale[8 * nt + 2 * t]);
-      if (!fold) {
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-          for (int mt = 0; mt < S::kMT; ++mt) {
-            const float f0 = col[nt].x * k_scale[mt * 16 / kSub], f1 = col[nt].y * k_scale[mt * 16 / kSub];
-            s[mt][nt][0] *= f0;
-            s[mt][nt][1] *= f1;
-            s[mt][nt][2] *= f0;
-            s[mt][nt][3] *= f1;
-          }
-        }
-      }
       if (partial) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
           const int2 end = *reinterpret_cast<const int2*>(&row_end[8 * nt + 2 * t]);
 #pragma unroll
           for (int mt = 0; mt < S::kMT; ++mt) {
+            const float f0 = col[nt].x * k_scale[mt * 16 / kSub], f1 = col[nt].y * k_scale[mt * 16 / kSub];
             const int token = there[mt * 16 / kSub] ? token0 + 16 * mt + token_of<kD>(g) : 0x7ffffff0;
-            if (token >= end.x) s[mt][nt][0] = kMinusInf;
-            if (token >= end.y) s[mt][nt][1] = kMinusInf;
-            if (token + 8 >= end.x) s[mt][nt][2] = kMinusInf;
-            if (token + 8 >= end.y) s[mt][nt][3] = kMinusInf;
+            s[mt][nt][0] = token < end.x ? s[mt][nt][0] * f0 : kMinusInf;
+            s[mt][nt][1] = token < end.y ? s[mt][nt][1] * f1 : kMinusInf;
+            s[mt][nt][2] = token + 8 < end.x ? s[mt][nt][2] * f0 : kMinusInf;
+            s[mt][nt][3] = token + 8 < end.y ? s[mt][nt][3] * f1 : kMinusInf;
           }
+          col[nt] = make_float2(1.0f, 1.0f);  // what is left to multiply by
         }
+#pragma unroll
+        for (int sub = 0; sub < S::kSubs; ++sub) k_scale[sub] = 1.0f;
       }
       float top[kNT][2];
       bool passed = false;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        float top0 = fmaxf(s[0][nt][0], s[0][nt][2]), top1 = fmaxf(s[0][nt][1], s[0][nt][3]);
+        float top0 = kMinusInf, top1 = kMinusInf;
+        constexpr int kSteps = kSub / 16;
 #pragma unroll
-        for (int mt = 1; mt < S::kMT; ++mt) {
-          top0 = fmaxf(top0, fmaxf(s[mt][nt][0], s[mt][nt][2]));
-          top1 = fmaxf(top1, fmaxf(s[mt][nt][1], s[mt][nt][3]));
+        for (int sub = 0; sub < S::kSubs; ++sub) {
+          float in0 = fmaxf(s[sub * kSteps][nt][0], s[sub * kSteps][nt][2]), in1 = fmaxf(s[sub * kSteps][nt][1], s[sub * kSteps][nt][3]);
+#pragma unroll
+          for (int mt = sub * kSteps + 1; mt < (sub + 1) * kSteps; ++mt) {
+            in0 = fmaxf(in0, fmaxf(s[mt][nt][0], s[mt][nt][2]));
+            in1 = fmaxf(in1, fmaxf(s[mt][nt][1], s[mt][nt][3]));
+          }
+          top0 = S::kSubs == 1 ? in0 : fmaxf(top0, in0 * k_scale[sub]);
+          top1 = S::kSubs == 1 ? in1 : fmaxf(top1, in1 * k_scale[sub]);
         }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
           top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
           top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
         }
-        col[nt].x = fold ? col[nt].x * k_scale[0] : 1.0f;  // what is left to multiply by
-        col[nt].y = fold ? col[nt].y * k_scale[0] : 1.0f;
-        top[nt][0] = top0 * col[nt].x;
-        top[nt][1] = top1 * col[nt].y;
+        top[nt][0] = top0 * (S::kSubs == 1 ? col[nt].x * k_scale[0] : col[nt].x);
+        top[nt][1] = top1 * (S::kSubs == 1 ? col[nt].y * k_scale[0] : col[nt].y);
         passed = passed || top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
       }
       if (__any_sync(0xffffffffu, passed)) {
@@ -660,32 +654,44 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) v_max = there[sub] ? fmaxf(v_max, v_scale[sub]) : v_max;
       bool plain = v_max <= kMaxFloat && v_max >= v_top * 0x1p-80f;
-      float share[S::kSubs];
-      const float inv_unit = S::kSubs > 1 ? 1.0f / v_max : 1.0f;
+      bool mixed = false;
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) {
-        if (S::kSubs > 1) plain = plain && (!there[sub] || v_scale[sub] >= v_max * 0.125f);
-        share[sub] = S::kSubs > 1 && there[sub] ? v_scale[sub] * inv_unit : 1.0f;
+        if (S::kSubs > 1) {
+          plain = plain && (!there[sub] || v_scale[sub] >= v_max * 0.125f);
+          mixed = mixed || (there[sub] && v_scale[sub] != v_max);
+        }
+      }
+      mixed = mixed && plain;
+      float share[S::kSubs];
+      if (S::kSubs > 1 && mixed) {
+        const float inv = 1.0f / v_max;
+#pragma unroll
+        for (int sub = 0; sub < S::kSubs; ++sub) share[sub] = there[sub] ? v_scale[sub] * inv : 1.0f;
       }
 #pragma unroll
-      for (int sub = 0; sub < S::kSubs; ++sub) share[sub] = plain ? share[sub] : 1.0f;
-#pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        const float e0 = col[nt].x, e1 = col[nt].y;
         // a column without a token so far: any finite reference will do
         const float ref0 = m[nt][0] == kMinusInf ? 0.0f : m[nt][0], ref1 = m[nt][1] == kMinusInf ? 0.0f : m[nt][1];
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
-          float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
-          float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
+          const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
+          const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
+          const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
-          if constexpr (S::kSubs > 1) {
-            const float f = share[mt * 16 / kSub];
-            p0 *= f, p1 *= f, p2 *= f, p3 *= f;
-          }
-          pf[mt][nt][0] = transpose8x8(half2_of(p0, p1));
-          pf[mt][nt][1] = transpose8x8(half2_of(p2, p3));
+          s[mt][nt][0] = p0, s[mt][nt][1] = p1, s[mt][nt][2] = p2, s[mt][nt][3] = p3;
+        }
+        if (S::kSubs > 1 && mixed) {
+#pragma unroll
+          for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][nt][e] *= share[mt * 16 / kSub];
+        }
+#pragma unroll
+        for (int mt = 0; mt < S::kMT; ++mt) {
+          pf[mt][nt][0] = transpose8x8(half2_of(s[mt][nt][0], s[mt][nt][1]));
+          pf[mt][nt][1] = transpose8x8(half2_of(s[mt][nt][2], s[mt][nt][3]));
         }
       }
       bool strange = false;
@@ -791,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 ? 3 : 2) kv_attention_kerne
 #pragma unroll
         for (int sub = 0; sub < S::kSubs; ++sub) {
           if (!there[sub]) continue;
-          const float f = v_scale[sub] / (plain ? v_unit * share[sub] : v_unit);  // p has its share already
+          const float f = (mixed ? v_max : v_scale[sub]) / v_unit;  // p may have its share of the largest already
           for (int end = max(lo, sub * kSub + 1); end <= hi; ++end) {
             product(std::true_type{}, sub, end, f, [&](int nt, int c) {
               return min(row_end[8 * nt + 2 * t + c] - token0, kChunk) == end;
@@ -1058,11 +1064,9 @@ template <int kD, int kSub>
 cudaError_t run_rows(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream) {
   // query rows that share a kv head, in an average sequence
   const long long rows = p.cu_seqlens == nullptr ? p.group : (static_cast<long long>(p.tokens) * p.group + p.batch - 1) / (p.batch > 0 ? p.batch : 1);
-  if (rows <= 8) return run_t<kD, 1, kSub>(p, bytes, stream);
-  if constexpr (kD <= 128) {
-    if (rows > 16) return run_t<kD, 4, kSub>(p, bytes, stream);
-  }
-  return run_t<kD, 2, kSub>(p, bytes, stream);
+  // 16 rows a tile (168 registers, three blocks an SM) beat 32 rows, which convert the codes half as often but leave room
+  // for two blocks: 32 requests of 1 to 6 tokens, 8 heads a kv head, 103 us against 119 (8 rows: 124).
+  return rows <= 8 ? run_t<kD, 1, kSub>(p, bytes, stream) : run_t<kD, 2, kSub>(p, bytes, stream);
 }
 
 }  // namespace

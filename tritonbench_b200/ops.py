@@ -343,6 +343,13 @@ def _raw_stream_slow(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream_slow)
 
 
+def _fresh_like(x: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor like x with its last dimension contiguous.  empty_like is the cheaper call, but of an
+    expanded x it may make an expanded dimension the innermost one."""
+    out = torch.empty_like(x)
+    return out if out.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, table, interleaved, transpose):
@@ -396,7 +403,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
             raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
         return _Rotary.apply(x, positions, table, interleaved, transpose)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+        out = _fresh_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != device or out.stride(2) != 1:
         raise ValueError("out must have x's shape, dtype and device, dim contiguous")
     if tokens == 0 or heads == 0:
@@ -530,12 +537,10 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
         if q_one != 1:
             raise ValueError("q must have head_dim contiguous")
         if q_out is None:
-            q_out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
-            o_token, o_head, fill = heads * dim, dim, 1
-        else:
-            if q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != device or q_out.stride(2) != 1:
-                raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
-            o_token, o_head, _ = q_out.stride()
+            q_out, fill = _fresh_like(q), 1
+        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != device or q_out.stride(2) != 1:
+            raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
+        o_token, o_head, _ = q_out.stride()
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
@@ -592,12 +597,10 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
         raise ValueError("q must have head_dim contiguous")
     fill = 0
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=dtype, device=q.device)
-        o_token, o_head, fill = heads * dim, dim, 1
-    else:
-        if out.shape != q.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
-            raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
-        o_token, o_head, _ = out.stride()
+        out, fill = _fresh_like(q), 1
+    elif out.shape != q.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
+        raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+    o_token, o_head, _ = out.stride()
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
     if tokens:
