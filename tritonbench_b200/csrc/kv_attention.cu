@@ -130,26 +130,19 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionParams& p, int b) {
 constexpr int kTileCost = 1;
 
 template <int kRows, int kUnit>
-__device__ __forceinline__ long long cost_of(const KvAttentionParams& p, int b) {
+__device__ __forceinline__ int cost_of(const KvAttentionParams& p, int b) {  // all sequences together: below 2^31
   const Seq s = seq_of<kRows, kUnit>(p, b);
-  return static_cast<long long>(s.row_tiles) * p.kv_heads * (s.units + kTileCost);
+  return s.row_tiles * p.kv_heads * (s.units + kTileCost);
 }
 
 // Equal shares of `total`: CTA c has [begin(c), begin(c + 1)).
 struct Shares {
-  long long each, rest;  // the first `rest` shares are one larger
-  __device__ __forceinline__ Shares(long long total, int ctas) {
-    if (total <= 0xffffffffll) {  // 64-bit division is slow
-      each = static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas);
-    } else {
-      each = total / ctas;
-    }
-    rest = total - each * ctas;
-  }
-  __device__ __forceinline__ long long begin(int c) const { return c * each + (c < rest ? c : rest); }
-  __device__ __forceinline__ int holder(long long at) const {  // CTA whose share `at` is in
-    const long long large = rest * (each + 1);
-    return static_cast<int>(at < large ? at / (each + 1) : rest + (at - large) / each);
+  int each, rest;  // the first `rest` shares are one larger
+  __device__ __forceinline__ Shares(int total, int ctas) : each(total / ctas) { rest = total - each * ctas; }
+  __device__ __forceinline__ int begin(int c) const { return c * each + min(c, rest); }
+  __device__ __forceinline__ int holder(int at) const {  // CTA whose share `at` is in
+    const int large = rest * (each + 1);
+    return at < large ? at / (each + 1) : rest + (at - large) / each;
   }
 };
 
@@ -176,7 +169,7 @@ struct Cursor {
   }
   // To the next unit, `left` being the rest of the share behind the present one, which becomes what is left behind the
   // cost of a tile that is entered.
-  __device__ __forceinline__ void advance(const KvAttentionParams& p, long long& left) {
+  __device__ __forceinline__ void advance(const KvAttentionParams& p, int& left) {
     if (++unit < s.units || left <= 0) return;
     left -= kTileCost;
     if (left <= 0) return;  // the share ends in front of the tile's first unit
@@ -235,11 +228,13 @@ __device__ __forceinline__ int token_of(int i) {
 template <int kRows, int kD>
 __host__ __device__ constexpr size_t part_floats() { return static_cast<size_t>(kRows) * (kD + 2); }
 
-struct alignas(16) Split {  // of CTA c
-  int first_cta;  // the CTA that began the tile inside which the share of c begins; -1: none
-  int last_cta;   // the CTA that finishes the tile which c began and did not finish; -1: none.  Then, of that tile:
+// A tile that CTAs first_cta to last_cta share (first_cta -1: none).
+struct SharedTile {
+  int first_cta, last_cta;
   int q_base, kv_head, row0, rows;
-  int pad[2];
+};
+struct alignas(16) Split {
+  SharedTile role[2];  // the tile inside which a CTA's share begins, the tile that it begins and does not finish
 };
 
 // q and out are bf16 or fp16: 16 bits an element either way
@@ -276,9 +271,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   using C = Cursor<S::kRows, S::kUnit>;
   constexpr int kChunk = S::kChunk, kStages = S::kStages;
   extern __shared__ __align__(128) char smem[];
-  __shared__ long long sums[kWarps];
-  __shared__ long long found_before;
-  __shared__ int found_b;
+  __shared__ int sums[kWarps], found_b, found_before;
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   const int g = lane >> 2, t = lane & 3;
   const int cta = static_cast<int>(blockIdx.x);
@@ -286,13 +279,13 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   float* parts = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + p.parts_offset);
 
   // ---- this CTA's share of the list
-  if (threadIdx.x == 0) splits[cta].first_cta = splits[cta].last_cta = -1;
-  long long total = 0, own = 0;
+  if (threadIdx.x == 0) splits[cta].role[0].first_cta = splits[cta].role[1].first_cta = -1;
+  int total = 0, own = 0;
   for (int b = threadIdx.x; b < p.batch; b += kThreads) own = cost_of<S::kRows, S::kUnit>(p, b), total += own;
-  long long upto = total;
+  int upto = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
   if (lane == 31) sums[warp] = upto;
@@ -304,30 +297,30 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     total += sums[w];
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid to complete
-  const int ctas = static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
+  const int ctas = min(total, static_cast<int>(gridDim.x));
   if (cta >= ctas) return;
   const Shares shares(total, ctas);
-  const long long run_begin = shares.begin(cta), run_end = shares.begin(cta + 1);
+  const int run_begin = shares.begin(cta), run_end = shares.begin(cta + 1);
   if (p.batch <= kThreads) {  // a thread has one sequence, and what lies in front of it
     if (run_begin >= upto - own && run_begin < upto) {
       found_b = threadIdx.x;
       found_before = upto - own;
     }
   } else {
-    long long before = 0;  // in front of b0
+    int before = 0;  // in front of b0
     for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
       const int b = b0 + static_cast<int>(threadIdx.x);
       own = b < p.batch ? cost_of<S::kRows, S::kUnit>(p, b) : 0;
       upto = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       __syncthreads();  // sums of the step before have been read
       if (lane == 31) sums[warp] = upto;
       __syncthreads();
-      long long step = 0;
+      int step = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w < warp) upto += sums[w];
@@ -347,20 +340,23 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   C cur;
   cur.b = found_b;
   cur.enter_sequence(p);
-  long long left = run_end - run_begin;  // of the share, from cur's unit on
+  int left = run_end - run_begin;  // of the share, from cur's unit on
   {
-    const long long in_seq = run_begin - found_before;
-    const int tile_cost = cur.s.units + kTileCost;
-    cur.tile = static_cast<int>(in_seq <= 0xffffffffll ? static_cast<uint32_t>(in_seq) / static_cast<uint32_t>(tile_cost) : in_seq / tile_cost);
-    const int in_tile = static_cast<int>(in_seq - static_cast<long long>(cur.tile) * tile_cost);
+    const int in_seq = run_begin - found_before, tile_cost = cur.s.units + kTileCost;
+    cur.tile = in_seq / tile_cost;
+    const int in_tile = in_seq - cur.tile * tile_cost;
     cur.unit = max(in_tile - kTileCost, 0);
     left -= max(kTileCost - in_tile, 0);
   }
   if (left <= 0) return;  // nothing but the cost of a tile
   cur.enter_tile(p);
-  if (threadIdx.x == 0 && cur.unit > 0) splits[cta].first_cta = shares.holder(run_begin - cur.unit);
+  if (threadIdx.x == 0 && cur.unit > 0) {
+    const int tile_begin = run_begin - cur.unit;
+    splits[cta].role[0] = {shares.holder(tile_begin), shares.holder(tile_begin + cur.s.units - 1), cur.s.q_base, cur.kv_head,
+                           cur.row0, min(S::kRows, cur.s.n * p.group - cur.row0)};
+  }
   C ahead = cur;
-  long long ahead_left = left;
+  int ahead_left = left;
 
   // ---- the ring of a warp: it copies and reads its own chunks, in step
   char* const ring = smem + warp * kStages * S::kStageBytes;
@@ -458,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   while (left > 0) {
     // ---- a segment: the units of this run that belong to one tile
     const int unit0 = cur.unit;
-    const int unit_end = static_cast<int>(min(static_cast<long long>(cur.s.units), unit0 + left));
+    const int unit_end = min(cur.s.units, unit0 + left);
     const int rows = min(S::kRows, cur.s.n * p.group - cur.row0);
     // queries to fp16, each row scaled by a power of two to a largest element in [1, 2); 16 elements a thread
     for (int i = threadIdx.x; i < S::kRows * (kD / 16); i += kThreads) {
@@ -877,11 +873,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     }
     if (begins && !ends && threadIdx.x == 0) {
       // the share ends with this segment, so the tile's last unit is as far behind the share's end as behind the segment's
-      splits[cta].last_cta = shares.holder(run_end + (cur.s.units - unit_end) - 1);
-      splits[cta].q_base = cur.s.q_base;
-      splits[cta].kv_head = cur.kv_head;
-      splits[cta].row0 = cur.row0;
-      splits[cta].rows = rows;
+      splits[cta].role[1] = {cta, shares.holder(run_end + (cur.s.units - unit_end) - 1), cur.s.q_base, cur.kv_head, cur.row0, rows};
     }
     __syncthreads();  // the warps' sums and the queries have been read
     left -= unit_end - unit0;
@@ -937,22 +929,26 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
       if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.heads + head] = kMinusInf;
     }
   }
-  const Split mine = splits[cta];
-#pragma unroll 1
-  for (int role = 0; role < 2; ++role) {  // the tile that this CTA continued, the tile that it began
-    const int first = role == 0 ? mine.first_cta : (mine.last_cta >= 0 ? cta : -1);
-    if (first < 0) continue;
-    const Split sp = role == 0 ? splits[first] : mine;
+  // half of the threads take the tile that this CTA continued, half the one that it began
+  constexpr int kThreadsOfRole = kJoinThreads / 2;
+  const int role = static_cast<int>(threadIdx.x) / kThreadsOfRole, thread = static_cast<int>(threadIdx.x) % kThreadsOfRole;
+  float4* const role_acc = group_acc + role * kThreadsOfRole;
+  float2* const role_ml = group_ml + role * kThreadsOfRole;
+  const auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + role), "n"(kThreadsOfRole) : "memory"); };
+  const SharedTile sp = splits[cta].role[role];
+  if (sp.first_cta < 0) return;
+  {
+    const int first = sp.first_cta;
     const int count = sp.last_cta - first + 1;
     // the beginning of the tile is part 1 of its CTA, what follows is part 0 of the next ones
     const auto part = [&](int i) { return parts + (2ll * (first + i) + (i == 0 ? 1 : 0)) * part_floats<kRows, kD>(); };
     const int vecs = sp.rows * kVecs;  // of the tile; this block's:
     const int begin = static_cast<int>(static_cast<long long>(vecs) * (cta - first) / count);
     const int end = static_cast<int>(static_cast<long long>(vecs) * (cta - first + 1) / count);
-    for (int at = begin; at < end; at += kJoinThreads) {
-      const int n = min(end - at, kJoinThreads);
-      const int groups = min(min(kJoinThreads / n, kGroups), count);
-      const int group = static_cast<int>(threadIdx.x) / n, vec = at + static_cast<int>(threadIdx.x) % n;
+    for (int at = begin; at < end; at += kThreadsOfRole) {
+      const int n = min(end - at, kThreadsOfRole);
+      const int groups = min(min(kThreadsOfRole / n, kGroups), count);
+      const int group = thread / n, vec = at + thread % n;
       const int r = vec / kVecs, d = vec % kVecs;
       RunningSum run = {kMinusInf, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
       if (group < groups) {
@@ -978,21 +974,21 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
         }
       }
       if (groups > 1) {
-        group_acc[threadIdx.x] = run.acc;
-        group_ml[threadIdx.x] = make_float2(run.top, run.sum);
-        __syncthreads();
+        role_acc[thread] = run.acc;
+        role_ml[thread] = make_float2(run.top, run.sum);
+        sync();
       }
       if (group == 0) {
         float ref = run.top;
-        for (int x = 1; x < groups; ++x) ref = fmaxf(ref, group_ml[threadIdx.x + x * n].x);
+        for (int x = 1; x < groups; ++x) ref = fmaxf(ref, role_ml[thread + x * n].x);
         run.move_to(ref);
         for (int x = 1; x < groups; ++x) {
-          const float2 ml = group_ml[threadIdx.x + x * n];
-          run.add(ml.x, ml.y, group_acc[threadIdx.x + x * n]);
+          const float2 ml = role_ml[thread + x * n];
+          run.add(ml.x, ml.y, role_acc[thread + x * n]);
         }
         store_row(p, sp.q_base, sp.kv_head, sp.row0 + r, 4 * d, run.acc, run.top, run.sum);
       }
-      if (groups > 1) __syncthreads();
+      if (groups > 1) sync();
     }
   }
 }
