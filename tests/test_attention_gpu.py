@@ -659,6 +659,55 @@ def test_attention_split_over_the_context(cuda_device, lens, new, kv, group):
         assert torch.equal(ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens, case.cu), got)
 
 
+def test_attention_of_many_ragged_sequences(cuda_device):
+    """More sequences than a block has threads, many without new tokens or without context."""
+    gen = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 90, (333,), generator=gen).tolist()
+    new = torch.randint(0, 4, (333,), generator=gen).tolist()
+    lens[5], new[5], lens[300] = 4000, 9, 2500
+    case = Case(lens, new, kv=2, group=3, dim=64, page=16)
+    _check_attention(case, case.randn(case.tokens + 5, 6, 64).bfloat16())
+    q, k, v = _qkv(case, extra=2)
+    _check_append(case, q, k, v, _table(5000, 64))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_append_and_attention_over_drawn_batches(cuda_device, seed):
+    import random
+
+    rng = random.Random(seed)
+    batch = rng.choice([1, 2, 7, 30])
+    lens = [rng.choice([0, 1, rng.randint(1, 40), rng.randint(1, 700), rng.choice([16, 32, 64, 128, 256, 512])]) for _ in range(batch)]
+    new = None if rng.random() < 0.4 else [rng.choice([0, 1, 1, 2, 5, 17, rng.randint(0, 150)]) for _ in range(batch)]
+    if new is not None and not sum(new):
+        new[0] = 3
+    dim = rng.choice([64, 128, 256])
+    case = Case(lens, new, kv=rng.choice([1, 2, 5]), group=rng.choice([1, 2, 7, 8, 9, 20]), dim=dim, page=rng.choice([16, 32, 64, 128]),
+                dtype=rng.choice([BF16, FP16]), seed=seed, layout=rng.choice(["heads", "tokens"]))
+    if rng.random() < 0.3:
+        case.block_table[rng.randrange(batch), rng.randrange(case.block_table.shape[1])] = -1
+    q, k, v = _qkv(case, extra=rng.choice([0, 3]) if new else 0)
+    rotated = _check_append(case, q, k, v, _table(1024, rng.choice([dim, 32])), interleaved=rng.random() < 0.5)
+    _check_attention(case, rotated)
+
+
+def test_attention_in_place_and_without_cache(cuda_device):
+    """out may be q; a cache without pages and a block table without columns leave nothing to see."""
+    from tritonbench_b200 import ops
+
+    case = Case([9000, 3, 700], [2, 1, 40], kv=2, group=4, dim=128, page=32)
+    q = case.randn(43, 8, 128).bfloat16()
+    want = _check_attention(case, q)
+    assert ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens, case.cu, out=q) is q
+    assert torch.equal(q, want)
+    none = ops.Fp8KvCache.empty(0, 2, 128, 32)
+    for cache, table in ((none, case.block_table), (case.cache, case.block_table[:, :0])):
+        out, lse = ops.fp8_kv_attention(q, cache, table, case.seq_lens, case.cu, return_lse=True)
+        assert not out.any() and (lse == -math.inf).all()
+        kv = q[:, :2]
+        assert torch.equal(ops.fp8_kv_append(q, kv, kv, cache, table, case.seq_lens, case.cu)[:3], q[:3])
+
+
 def test_cache_of_more_than_2_to_the_32_bytes(cuda_device):
     """Pages whose byte offsets pass 32 bits, appended to and read."""
     from tritonbench_b200 import ops

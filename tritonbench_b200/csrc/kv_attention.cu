@@ -417,8 +417,9 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
               const int row = sub * kSub + n * kCopyRows;
               const uint32_t to = base + copy_at[n % kPlaces] + row / 8 * k8Rows;
               const bool take = whole.value || n * kCopyRows + copy_row < left;
-              copy_async<16, whole.value>(to, take ? k + n * kCopyRows * k_row : p.k_cache, take);
-              copy_async<16, whole.value>(to + S::kTileBytes, take ? v + n * kCopyRows * v_row : p.v_cache, take);
+              // (an address that is never read, and there even when the cache has no page)
+              copy_async<16, whole.value>(to, take ? static_cast<const void*>(k + n * kCopyRows * k_row) : p.workspace, take);
+              copy_async<16, whole.value>(to + S::kTileBytes, take ? static_cast<const void*>(v + n * kCopyRows * v_row) : p.workspace, take);
             }
           }
         };

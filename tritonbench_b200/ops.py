@@ -422,8 +422,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
 
 class Fp8KvCache:
     """A paged key/value cache in e4m3: k and v [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn (any page, head
-    and row strides that are multiples of 16; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads] float32;
-    a value is code * scale.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object describes the four tensors
+    and row strides that are multiples of 16 and below 2^31; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads] float32;
+    a value is code * scale, no scale is negative.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object describes the four tensors
     and keeps them alive; make one with `empty`, or around tensors of your own."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor")
@@ -509,7 +509,8 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     448.  A page that already holds tokens keeps its scale, or is moved to a larger one.  Infinities and NaN are stored as
     NaN.  Rows whose position would be negative (seq_lens[b] = 0: a padded entry), positions behind the block table and
     pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q) keeps its rows
-    behind cu_seqlens[-1]; in a fresh result they are zero.  Two sequences must not append to the same page."""
+    behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to twice in one call (two sequences
+    that share one, or a sequence that has it twice)."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
     device, heads, dim = cache.device, cache.kv_heads, cache.head_dim
@@ -572,7 +573,7 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     (a decode step, drafted tokens, a chunk of a prompt).  q [tokens, heads, head_dim] bf16 or fp16; heads / kv_heads
     neighbouring query heads share a kv head; block_table, seq_lens, cu_seqlens as for fp8_kv_append, which has stored the
     tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
-    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads].
+    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads].  out may be q.
 
     Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
     (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows behind
