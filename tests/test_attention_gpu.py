@@ -261,7 +261,9 @@ def _plain_store(codes, scales, x, case, old_codes, old_scales):
         rows = torch.tensor([r for _, r in members], device="cuda")
         y = x[rows]  # [n, kv, dim]
         amax = torch.where(y.isfinite(), y.abs(), 0.0).amax(dim=(0, 2)).double()
-        need = torch.where(amax > 0, torch.exp2(torch.ceil(torch.log2(amax / 448))), 0.0).clamp(min=2.0**-126)
+        fraction, exponent = torch.frexp(amax)  # 448 = 0.875 * 2^9; exact, where log2 of a power of two need not be
+        need = torch.ldexp(torch.ones_like(amax), torch.where(fraction <= 0.875, exponent - 9, exponent - 8)).clamp(min=2.0**-126)
+        need = torch.where(amax > 0, need, 2.0**-126)
         scale = torch.maximum(need, old_scales[page].double()) if held else need
         if held:
             moved = old_codes[page, :, :held].float() * (old_scales[page].double() / scale).float()[:, None, None]
@@ -378,6 +380,19 @@ def test_appended_page_grows_its_scale_step_by_step(cuda_device):
         # steps double: in all less than two half steps
         assert (off <= 2.0**-4 * x.abs() + 2 * 2.0**-10 * scale).all()
     assert lens == [1]
+
+
+def test_append_of_a_maximum_that_fills_the_format_exactly(cuda_device):
+    """448 * 2^e needs the scale 2^e and becomes the largest code; the next value above it needs twice that."""
+    case = Case([4, 4], [4, 4], kv=1, group=1, dim=64, page=16)
+    q, k, v = (t.clone() for t in _qkv(case, scale=0.01))
+    k[:4], k[4:], v[:4], v[4:] = 0.0, 0.0, 0.0, 0.0
+    k[1, 0, 3], k[5, 0, 3], v[2, 0, 0], v[6, 0, 0] = 7.0, -7.03125, -448.0, 450.0
+    _check_append(case, q, k, v)
+    first, second = (int(p) for p in case.block_table[:, 0])
+    assert case.ks[[first, second], 0].tolist() == [2.0**-6, 2.0**-5]
+    assert case.vs[[first, second], 0].tolist() == [1.0, 2.0]
+    assert case.k.view(torch.uint8)[first, 0, 1, 3] == 0x7E and case.v.view(torch.uint8)[first, 0, 2, 0] == 0xFE
 
 
 def test_append_of_values_that_do_not_count(cuda_device):
