@@ -305,6 +305,8 @@ int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, 
  * -infinity behind the last sequence.
  * (tokens * heads / kv_heads / 8 + batch) * kv_heads * (table_width * page_size / 64 + 2) must be below 2^31.
  * The workspace needs no initialisation and may be reused as soon as the call has run; calls that overlap need one each.
+ * Small calls need none: b200fp8_kv_attention_workspace_bytes is 0 then (also where the call itself would return an
+ * error), and workspace may be NULL.
  */
 size_t b200fp8_kv_attention_workspace_bytes(const b200fp8_kv_cache* cache, const b200fp8_kv_batch* rows, int64_t heads);
 int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_t heads, int64_t q_token, int64_t q_head,

@@ -66,7 +66,7 @@ def test_attention_refuses_bad_arguments(cdll, ptr):
     def call(q=ptr, out=ptr, dtype=0, heads=4, q_token=256, o_token=256, cache=_cache(ptr), rows=_rows(ptr), ws=ptr):
         return cdll.b200fp8_kv_attention(q, out, None, dtype, heads, q_token, 64, o_token, 64, cache, rows, 0.125, 0, ws, 16, None)
 
-    for kw in (dict(q=None), dict(out=None), dict(ws=None), dict(dtype=2), dict(heads=5), dict(cache=None), dict(rows=None),
+    for kw in (dict(q=None), dict(out=None), dict(dtype=2), dict(heads=5), dict(cache=None), dict(rows=None),
                dict(rows=_rows(ptr, tokens=2)), dict(rows=_rows(0))):
         assert call(**kw) == lib.BAD_ARG, kw
     for kw in (dict(q=ptr + 8), dict(out=ptr + 4), dict(q_token=260), dict(o_token=258), dict(ws=ptr + 8),

@@ -13,6 +13,7 @@ bf16 2^-8, fp32 2^-24), or half of the type's smallest subnormal.
              |do| <= (4 dsmax + 2^-11 + 2^-20 + N 2^-22 + 2^-22 |s|max) * sum_j w_j |v_j| + 2^-25 * sum_j |v_j|,
              plus half a step of the output.
 """
+import copy
 import math
 
 import pytest
@@ -225,6 +226,13 @@ class Case:
         if new is None:
             self.new = [1] * len(lens)
         self.tokens = sum(self.new)
+
+    def widen(self):
+        """A block table with room for far longer contexts: the call then goes by the list of units that long contexts
+        take, and not by one cluster of blocks per tile."""
+        columns = 20_000 // self.page
+        self.block_table = torch.cat([self.block_table, torch.full((len(self.lens), columns), -1, dtype=torch.int32, device="cuda")], 1)
+        return self
 
     def randn(self, *shape):
         return torch.randn(*shape, generator=self.gen, device="cuda")
@@ -520,8 +528,15 @@ def _plain_attention(case, q, softmax_scale):
 def _check_attention(case, q, softmax_scale=None, **kw):
     from tritonbench_b200 import ops
 
+    want, want_lse, bound, lse_bound = _plain_attention(case, q.clone(), case.dim**-0.5 if softmax_scale is None else softmax_scale)
+    wide = ops.fp8_kv_attention(q, case.cache, Case.widen(copy.copy(case)).block_table, case.seq_lens, case.cu, softmax_scale, return_lse=True)
+    _within(case, *wide, want, want_lse, bound, lse_bound)
     got, lse = ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens, case.cu, softmax_scale, return_lse=True, **kw)
-    want, want_lse, bound, lse_bound = _plain_attention(case, q, case.dim**-0.5 if softmax_scale is None else softmax_scale)
+    _within(case, got, lse, want, want_lse, bound, lse_bound)
+    return got
+
+
+def _within(case, got, lse, want, want_lse, bound, lse_bound):
     n = case.tokens
     off = (got[:n].double() - want[:n]).abs()
     limit = bound[:n] + _half_step(got.dtype) * (want[:n].abs() + bound[:n]) + TINY[got.dtype]
@@ -530,7 +545,7 @@ def _check_attention(case, q, softmax_scale=None, **kw):
     assert torch.equal(lse[:n] == -math.inf, empty)
     assert ((lse[:n].double() - want_lse[:n]).abs()[~empty] <= lse_bound[:n][~empty]).all()
     assert not got[:n][empty].any()
-    return got
+    assert not lse[n:].isfinite().any()
 
 
 LENS = [([1], None), ([2], None), ([15], None), ([16], None), ([17], None), ([31, 32, 33, 0, 127, 128, 129], None), ([777], None),
@@ -546,9 +561,12 @@ def test_attention_matches_64_bits(cuda_device, lens, new, kv, group, dim, page,
     _check_attention(case, case.randn(case.tokens, kv * group, dim).to(dtype))
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
-def test_attention_on_views(cuda_device, layout):
+def test_attention_on_views(cuda_device, layout, wide):
     case = Case([500, 90, 64], [2, 1, 6], kv=2, group=3, dim=64, page=32, layout=layout)
+    if wide:
+        case.widen()
     wide = case.randn(case.tokens + 3, 10 * 64).bfloat16().unflatten(1, (10, 64))
     out = torch.full((6, case.tokens + 3, 68), 5.0, device="cuda", dtype=BF16)[..., :64].transpose(0, 1)
     got = _check_attention(case, wide[:, 2:8], out=out)
@@ -571,10 +589,13 @@ def test_attention_with_queries_out_of_fp16_range(cuda_device, size):
     _check_attention(case, q, softmax_scale=0.125 / size)
 
 
-def test_attention_does_not_read_behind_a_sequence(cuda_device):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_does_not_read_behind_a_sequence(cuda_device, wide):
     """NaN codes and scales that are not finite everywhere the sequences do not reach, in their own last pages too."""
     lens = [70, 1, 128, 0, 31]
     case = Case(lens, None, kv=2, group=4, dim=64, page=64)
+    if wide:
+        case.widen()
     q = case.randn(5, 8, 64).bfloat16()
     want = _check_attention(case, q)
     used = torch.zeros(case.k.shape[0], 64, dtype=torch.bool, device="cuda")
@@ -593,13 +614,16 @@ def test_attention_does_not_read_behind_a_sequence(cuda_device):
     assert torch.equal(ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens), want)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("group,page,dim", [(1, 16, 64), (4, 64, 128), (8, 32, 128), (3, 128, 256)])
-def test_attention_keeps_later_tokens_nan_out_of_earlier_rows(cuda_device, group, page, dim):
+def test_attention_keeps_later_tokens_nan_out_of_earlier_rows(cuda_device, group, page, dim, wide):
     """A NaN in a key or value that only the later of a sequence's new tokens see."""
     from tritonbench_b200 import ops
 
     new = 7
     case = Case([page + 5, 40], [new, new], kv=2, group=group, dim=dim, page=page)
+    if wide:
+        case.widen()
     q = case.randn(case.tokens, 2 * group, dim).bfloat16()
     want = _check_attention(case, q)
     for codes in (case.v, case.k):
@@ -634,10 +658,13 @@ def test_attention_keeps_later_tokens_nan_out_of_earlier_rows(cuda_device, group
     assert torch.equal(got[keep], want[keep]) and not got[new - 1].isfinite().any() and pos > 0
 
 
-def test_attention_of_a_query_that_is_not_finite_stays_in_its_row(cuda_device):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_of_a_query_that_is_not_finite_stays_in_its_row(cuda_device, wide):
     from tritonbench_b200 import ops
 
     case = Case([300], [3], kv=1, group=5, dim=64, page=64)
+    if wide:
+        case.widen()
     q = case.randn(3, 5, 64).bfloat16()
     want = _check_attention(case, q)
     q[1, 2, 7], q[2, 0, 0] = float("nan"), float("inf")
@@ -764,7 +791,7 @@ def test_attention_refuses(cuda_device):
 def test_calls_on_two_streams_at_once(cuda_device):
     from tritonbench_b200 import ops
 
-    cases = [Case([3000 + 700 * i, 50], None, kv=2, group=8, dim=128, page=64, seed=i) for i in range(2)]
+    cases = [Case([3000 + 700 * i, 50], None, kv=2, group=8, dim=128, page=64, seed=i).widen() for i in range(2)]
     qs = [c.randn(2, 16, 128).bfloat16() for c in cases]
     want = [ops.fp8_kv_attention(q, c.cache, c.block_table, c.seq_lens) for c, q in zip(cases, qs)]
     torch.cuda.synchronize()
@@ -787,7 +814,7 @@ def test_a_captured_decode_step_follows_its_lengths(cuda_device):
     cases = [Case([900, 63, 0, 200], None, kv=2, group=4, dim=128, page=64, seed=s, spare=9) for s in range(2)]
     state, graphs = [], []
     for c in cases:
-        room = torch.full((4, 20), -1, dtype=torch.int32, device="cuda")
+        room = torch.full((4, 20 + 300 * cases.index(c)), -1, dtype=torch.int32, device="cuda")
         room[:, : c.block_table.shape[1]] = c.block_table
         spare = sorted(set(range(c.k.shape[0])) - set(c.block_table.flatten().tolist()))
         room[1, 1], room[3, 4], room[0, 15] = spare[0], spare[1], spare[2]

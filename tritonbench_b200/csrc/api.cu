@@ -1065,7 +1065,7 @@ int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_
   if (st != B200FP8_OK) return st;
   if (dtype != kQuantBf16 && dtype != kQuantFp16) return B200FP8_BAD_ARG;
   if (rows->tokens == 0) return B200FP8_OK;
-  if (q == nullptr || out == nullptr || workspace == nullptr) return B200FP8_BAD_ARG;
+  if (q == nullptr || out == nullptr) return B200FP8_BAD_ARG;
   if (!aligned16(q) || (q_token | q_head) % 8 != 0 || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
       (o_token | o_head) % 4 != 0 || !aligned16(workspace)) {
     return B200FP8_UNSUPPORTED_ALIGNMENT;
@@ -1077,6 +1077,7 @@ int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_
   const int sized = note_cuda(launch_kv_attention(p, &need, nullptr));
   if (sized != B200FP8_OK) return sized;
   if (workspace_bytes < need) return B200FP8_WORKSPACE_TOO_SMALL;
+  if (need > 0 && workspace == nullptr) return B200FP8_BAD_ARG;
   p.q = q;
   p.out = out;
   p.lse = lse;

@@ -14,7 +14,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.cu", "gemm_tc.cu", "gemm_skinny.cu", "gemm_simt.cu", "quantize.cu", "fused_quantize.cu", "gemm_splitk.cu", "gemm_blockwise.cu", "gemm_gemv.cu",
            "rotary.cu", "kv_append.cu", "kv_attention.cu"]
-HEADERS = ["ptx.cuh", "kernels.h", "streamk.cuh", "nanmax.cuh", "rotary.cuh", os.path.join("..", "..", "include", "b200fp8.h")]
+HEADERS = ["ptx.cuh", "kernels.h", "streamk.cuh", "nanmax.cuh", "rotary.cuh", "sequences.cuh", os.path.join("..", "..", "include", "b200fp8.h")]
 LIB_NAME = "libb200fp8.so"
 
 

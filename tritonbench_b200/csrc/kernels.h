@@ -350,8 +350,9 @@ struct KvAttentionParams {
   float softmax_scale;
   void* workspace;
   size_t workspace_bytes, parts_offset;
+  int cluster;  // CTAs of a tile, small calls (filled in by the launch)
 };
-// bytes != null: only says how large a workspace this call needs
+// bytes != null: only says how large a workspace this call needs; 0: none
 cudaError_t launch_kv_attention(const KvAttentionParams& p, size_t* bytes, cudaStream_t stream);
 
 }  // namespace b200fp8

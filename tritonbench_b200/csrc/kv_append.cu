@@ -21,29 +21,13 @@
 
 #include "kernels.h"
 #include "rotary.cuh"
+#include "sequences.cuh"
 
 namespace b200fp8 {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kN = 8;  // elements of a 16-byte vector of bf16 or fp16; a slot is two of them
-
-// Sequence of a packed index: the largest b with key(b) <= at, by all lanes of a warp, 32 candidates a step.
-// key is not decreasing, key(0) <= at.
-template <typename Key>
-__device__ __forceinline__ int search_sequence(int batch, long long at, const Key& key) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = batch;  // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int b = lo + lane * step;
-    const bool below = lane * step < n && key(b) <= at;
-    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1);
-    n = min(step, n - last * step);
-    lo += last * step;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);

@@ -610,11 +610,11 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
                 return fp8_kv_attention(q, cache, block_table, seq_lens, cu_seqlens, softmax_scale, None if fill else out, return_lse)
         lib = _lib.load()
         nbytes = lib.b200fp8_kv_attention_workspace_bytes(cache.descriptor, rows, heads)
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None  # small calls need none
         status = lib.b200fp8_kv_attention(
             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), _DTYPES[dtype], heads, q_token, q_head,
             o_token, o_head, cache.descriptor, rows, dim ** -0.5 if softmax_scale is None else softmax_scale, fill,
-            ws.data_ptr(), nbytes, _raw_stream(device))
+            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(device))
         if status:
             _lib.check(status, f"b200fp8_kv_attention(tokens={tokens}, heads={heads}, kv_heads={cache.kv_heads}, dim={dim})")
     return (out, lse) if return_lse else out
