@@ -1101,7 +1101,7 @@ struct Plan {
 };
 
 // CTAs of a grid that fills the current device once, per device (the same whoever asks first)
-constexpr int kSmallUnits = 6;
+constexpr int kSmallUnits = 4;
 
 template <int kD, int kNT, int kSub>
 cudaError_t make_plan(Plan* plan) {
@@ -1141,16 +1141,17 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
   cudaError_t err = make_plan<kD, kNT, kSub>(&plan);
   if (err != cudaSuccess) return err;
   KvAttentionParams p = params;
-  // A cluster per tile when the largest context that the block table allows leaves a CTA at most kSmallUnits units: up to
-  // 8 CTAs a tile, as long as all are resident at once.  It saves the second launch, the workspace and the list, about 3 us
-  // on the device and 5 on the host (1 x 777 tokens, 8 kv heads: 7.9 -> 5.1 us, the call 16.2 -> 11.0), but shares nothing
-  // between tiles, so long and ragged contexts go by the list.
+  // A cluster per tile when all of them are resident at once and the largest context that the block table allows leaves a
+  // CTA at most kSmallUnits units, up to 8 CTAs a tile.  It saves the second launch, the workspace and the list, about 2 us
+  // on the device and 5 on the host, but shares nothing between tiles.  Device us, list / clusters: 1 sequence of 1024
+  // tokens, 8 kv heads 8.0 / 5.9, of 4096 9.3 / 10.0 (4 units a CTA; the host takes 15.9 / 10.6), of 8192 11.1 / 14.8;
+  // 16 of 1024 13.6 / 12.4, of 2048 18.4 / 17.8 (ragged 14.3 / 17.5); 64 of 256, two waves, 14.7 / 17.8.
   const long long row_slots = p.cu_seqlens == nullptr ? static_cast<long long>(p.batch) * ((p.group + S::kRows - 1) / S::kRows)
                                                       : static_cast<long long>(p.tokens) * p.group / S::kRows + p.batch;
   const long long tiles = row_slots * p.kv_heads, units = p.max_len > S::kUnit ? (p.max_len + S::kUnit - 1) / S::kUnit : 1;
   p.cluster = kMaxCluster;
   while (p.cluster > 1 && (tiles * p.cluster > plan.ctas || p.cluster / 2 >= units)) p.cluster /= 2;
-  const bool clustered = (tiles * p.cluster + plan.ctas - 1) / plan.ctas * ((units + p.cluster - 1) / p.cluster) <= kSmallUnits;
+  const bool clustered = tiles * p.cluster <= plan.ctas && units <= kSmallUnits * p.cluster;
   if (bytes != nullptr) {  // only asked for the size
     *bytes = clustered ? 0 : plan.bytes;
     return cudaSuccess;
