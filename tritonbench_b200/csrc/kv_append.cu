@@ -19,6 +19,8 @@
 // between the maximum and the codes.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "rotary.cuh"
 #include "sequences.cuh"
@@ -46,14 +48,15 @@ __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
 }
 __device__ __forceinline__ float nan_for_inf(float v) { return fabsf(v) <= 3.402823466e38f ? v : __int_as_float(0x7fffffff); }
 
-__device__ __forceinline__ uint2 codes8(const float (&y)[kN], float inv) {
-  uint32_t w[2];
+__device__ __forceinline__ uint2 codes8(const float (&y)[kN], float inv, bool infinite) {
+  float z[kN];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    w[i] = codes2(nan_for_inf(y[4 * i]) * inv, nan_for_inf(y[4 * i + 1]) * inv) |
-           (codes2(nan_for_inf(y[4 * i + 2]) * inv, nan_for_inf(y[4 * i + 3]) * inv) << 16);
+  for (int i = 0; i < kN; ++i) z[i] = y[i] * inv;
+  if (infinite) {  // the conversion would saturate it; a NaN stays one by itself
+#pragma unroll
+    for (int i = 0; i < kN; ++i) z[i] = nan_for_inf(z[i]);
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(codes2(z[0], z[1]) | (codes2(z[2], z[3]) << 16), codes2(z[4], z[5]) | (codes2(z[6], z[7]) << 16));
 }
 
 __device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
@@ -157,15 +160,15 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   };
   uint8_t* codes = nullptr;
   const long long code_row = p.cache_row[which];
+  bool infinite = false;  // among the group's values
   const auto store = [&](int item, const float (&a)[kN], const float (&c)[kN], float inv) {
     const int row = item / slots;
     const SlotAt at = slot_at<kInterleaved>(item - row * slots, rot);
     uint8_t* r = codes + (held + row) * code_row;
-    *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv);
-    *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv);
+    *reinterpret_cast<uint2*>(r + at.a) = codes8(a, inv, infinite);
+    *reinterpret_cast<uint2*>(r + at.b) = codes8(c, inv, infinite);
   };
 
-  float amax = 0.0f;
   float ka[kHold][kN], kb[kHold][kN];
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
@@ -175,31 +178,41 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   codes = (which ? p.v_cache : p.k_cache) + page * p.cache_page[which] + head * p.cache_head[which];
   float* const scale_at = (which ? p.v_scale : p.k_scale) + page * p.scale_page[which] + head * p.scale_head[which];
   const float old_scale = held > 0 ? *scale_at : 0.0f;
+  // largest magnitude; fmaxf passes over NaN, an infinity is looked for only when there is one
+  const auto largest = [&](auto finite_only) {
+    const auto take = [&](float v) { return finite_only.value ? finite_abs(v) : fabsf(v); };
+    float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kHold; ++i) {
-    if (in_group + i * kGroup < items) {
+    for (int i = 0; i < kHold; ++i) {
+      if (in_group + i * kGroup < items) {
 #pragma unroll
-      for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(finite_abs(ka[i][e]), finite_abs(kb[i][e])));
+        for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(take(ka[i][e]), take(kb[i][e])));
+      }
     }
-  }
-  for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
-    float a[kN], c[kN];
-    load(item, a, c);
+    for (int item = in_group + kHold * kGroup; item < items; item += kGroup) {
+      float a[kN], c[kN];
+      load(item, a, c);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(finite_abs(a[e]), finite_abs(c[e])));
-  }
+      for (int e = 0; e < kN; ++e) amax = fmaxf(amax, fmaxf(take(a[e]), take(c[e])));
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if constexpr (kGroup > 32) {
-    __shared__ float red[kThreads / 32];
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    __syncthreads();
-    amax = red[0];
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if constexpr (kGroup > 32) {
+      __shared__ float red[kThreads / 32];
+      __syncthreads();  // red of a first pass has been read
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+      __syncthreads();
+      amax = red[0];
 #pragma unroll
-    for (int w = 1; w < kGroup / 32; ++w) amax = fmaxf(amax, red[w]);
-  } else {
-    __syncwarp();  // every lane has read the old scale before lane 0 writes the new one
-  }
+      for (int w = 1; w < kGroup / 32; ++w) amax = fmaxf(amax, red[w]);
+    } else {
+      __syncwarp();  // every lane has read the old scale before lane 0 writes the new one
+    }
+    return amax;
+  };
+  float amax = largest(std::false_type{});
+  infinite = !(amax <= 3.402823466e38f);  // the same for the whole group
+  if (infinite) amax = largest(std::true_type{});
   const float need = pow2_scale(amax);
   const float scale = fmaxf(old_scale, need);
   const float inv = __fdiv_rn(1.0f, scale);

@@ -288,6 +288,7 @@ __device__ __forceinline__ void fill_behind(const KvAttentionParams& p, int thre
 }
 
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the aligned forms want whole warps
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {  // the same shared memory of another CTA of the cluster
@@ -1036,10 +1037,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   const int role = static_cast<int>(threadIdx.x) / kThreadsOfRole, thread = static_cast<int>(threadIdx.x) % kThreadsOfRole;
   float4* const role_acc = group_acc + role * kThreadsOfRole;
   float2* const role_ml = group_ml + role * kThreadsOfRole;
-  const auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + role), "n"(kThreadsOfRole) : "memory"); };
+  const auto sync = [&]() {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + role), "n"(kThreadsOfRole) : "memory");
+  };
   const SharedTile sp = splits[cta].role[role];
-  if (sp.first_cta < 0) return;
-  {
+  if (sp.first_cta >= 0) {
     const int first = sp.first_cta;
     const int count = sp.last_cta - first + 1;
     // the beginning of the tile is part 1 of its CTA, what follows is part 0 of the next ones
