@@ -10,13 +10,14 @@
 //     half of a 16-row tile.  O^T = V^T P^T then has the head dimension as rows, and P^T goes from accumulator to
 //     operand layout with one movmatrix per 8 tokens.
 //   * e4m3 is exact in fp16, and so are bf16 queries once a row is scaled by a power of two (what falls below fp16's
-//     range then is under 2^-24 of the row's largest element); p <= 1 rounded to fp16 is off by 2^-12.  tcgen05 takes
-//     8-bit operands only in pairs, which would round queries and p to 3 bits of mantissa.  Sums, maxima and the
-//     output stay in fp32.
+//     range then is under 2^-24 of the row's largest element); p rounded to fp16 is off by 2^-11 of itself at most.
+//     tcgen05 takes 8-bit operands only in pairs, which would round queries and p to 3 bits of mantissa.  Sums, maxima
+//     and the output stay in fp32.
 //   * The order of the contraction is free, so a thread's operand elements are 16 neighbouring bytes of a token:
 //     whole 16-byte vectors are loaded, and the pairing of two tokens' V bytes costs one byte permute per 4 bytes.
 //     A warp copies (cp.async, whole rows) and reads its own chunks, so the ring needs no barrier beyond the warp.
-//   * v_scale differs by page: O is kept in units of the V scale that was added last, so products accumulate in place.
+//   * v_scale differs by page: O is kept in units of the largest V scale of the chunk that was added last, so products
+//     accumulate in place.
 // Work is split over the context: all (sequence, kv head, row tile, unit of 4 chunks) units of the batch are one list,
 // cut into equal runs for a grid that fills the GPU once; lengths are read on the device.  A run that ends inside a
 // tile leaves its unnormalised sums in the workspace (at most two parts a CTA) and the second kernel joins them, in a
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     cur.unit = cur.s.units * rank / p.cluster;
     left = cur.s.units * (rank + 1) / p.cluster - cur.unit;
   } else {
-    if (threadIdx.x == 0) splits[cta].role[0].first_cta = splits[cta].role[1].first_cta = -1;
+    if (threadIdx.x == 0) splits[cta].role[0].first_cta = splits[cta].role[1].first_cta = found_b = -1;
     int total = 0, own = 0;
     for (int b = threadIdx.x; b < p.batch; b += kThreads) own = cost_of<S::kRows, S::kUnit>(p, b), total += own;
     int upto = total;
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     }
     __syncthreads();
 
+    if (found_b < 0) return;  // bounds that run backwards and count rows more than once: the sum may have wrapped
     cur.b = found_b;
     cur.enter_sequence(p);
     left = run_end - run_begin;
