@@ -303,7 +303,7 @@ int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, 
  * fp16, element pitches multiples of 8 (out: of 4); lse [tokens, heads] fp32 (natural logarithm of the softmax's
  * denominator) or NULL.  A row without a token to see gives zeros, and lse = -infinity.  fill_rest as above for out; lse is
  * -infinity behind the last sequence.
- * (tokens * heads / kv_heads / 8 + batch) * kv_heads * (table_width * page_size / 64 + 2) must be below 2^31.
+ * (tokens * heads / kv_heads / 8 + batch) * kv_heads * (table_width * page_size / 64 + 3) must be below 2^31.
  * The workspace needs no initialisation and may be reused as soon as the call has run; calls that overlap need one each.
  * Small calls need none: b200fp8_kv_attention_workspace_bytes is 0 then (also where the call itself would return an
  * error), and workspace may be NULL.

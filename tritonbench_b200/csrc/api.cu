@@ -1072,7 +1072,7 @@ int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_
   }
   KvAttentionParams p = kv_attention_params(*cache, *rows, heads);
   // the kernel counts pieces of at least 64 tokens by 8 query rows in 32 bits
-  if ((static_cast<double>(p.tokens) * p.group / 8 + p.batch) * p.kv_heads * (p.max_len / 64.0 + 2) > 2147483647.0) return B200FP8_TOO_LARGE;
+  if ((static_cast<double>(p.tokens) * p.group / 8 + p.batch) * p.kv_heads * (p.max_len / 64.0 + 3) > 2147483647.0) return B200FP8_TOO_LARGE;
   size_t need = 0;
   const int sized = note_cuda(launch_kv_attention(p, &need, nullptr));
   if (sized != B200FP8_OK) return sized;

@@ -130,14 +130,17 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionParams& p, int b) {
   return s;
 }
 // Cost of a tile besides its units, in units: loading the queries, joining the warps and storing what they found takes a
-// block about 2.3 us, a unit takes it 2.0 us (three blocks an SM, the memory busy).  Runs of equal units without it ended
-// between 67 and 98 us (64 sequences of 1 to 8192 tokens), those with eleven tiles last.
-constexpr int kTileCost = 1;
+// block 2 to 3 us, a unit takes it 2.0 us (three blocks an SM, the memory busy).  Shares of equal units without it ended
+// between 67 and 98 us (64 sequences of 1 to 8192 tokens), those with eleven tiles last.  Device us for a cost of 1 / 2 / 3:
+// those 95.1 / 93.5 / 94.5, drafted tokens 102.5 / 95.7 / 96.6; 48 sequences with heads of 64, whose tiles are half as
+// large, 67.0 / 68.1 / 71.8.
+template <int kUnit>
+__host__ __device__ constexpr int tile_cost() { return kUnit >= 256 ? 1 : 2; }
 
 template <int kRows, int kUnit>
 __device__ __forceinline__ int cost_of(const KvAttentionParams& p, int b) {  // all sequences together: below 2^31
   const Seq s = seq_of<kRows, kUnit>(p, b);
-  return s.row_tiles * p.kv_heads * (s.units + kTileCost);
+  return s.row_tiles * p.kv_heads * (s.units + tile_cost<kUnit>());
 }
 
 // Equal shares of `total`: CTA c has [begin(c), begin(c + 1)).
@@ -176,7 +179,7 @@ struct Cursor {
   // cost of a tile that is entered.
   __device__ __forceinline__ void advance(const KvAttentionParams& p, int& left) {
     if (++unit < s.units || left <= 0) return;
-    left -= kTileCost;
+    left -= tile_cost<kUnit>();
     if (left <= 0) return;  // the share ends in front of the tile's first unit
     unit = 0;
     if (++tile == s.row_tiles * p.kv_heads) {
@@ -416,11 +419,12 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     cur.enter_sequence(p);
     left = run_end - run_begin;
     {
-      const int in_seq = run_begin - found_before, tile_cost = cur.s.units + kTileCost;
-      cur.tile = in_seq / tile_cost;
-      const int in_tile = in_seq - cur.tile * tile_cost;
-      cur.unit = max(in_tile - kTileCost, 0);
-      left -= max(kTileCost - in_tile, 0);
+      constexpr int kCost = tile_cost<S::kUnit>();
+      const int in_seq = run_begin - found_before, of_tile = cur.s.units + kCost;
+      cur.tile = in_seq / of_tile;
+      const int in_tile = in_seq - cur.tile * of_tile;
+      cur.unit = max(in_tile - kCost, 0);
+      left -= max(kCost - in_tile, 0);
     }
     if (left <= 0) return;  // nothing but the cost of a tile
     cur.enter_tile(p);
