@@ -317,18 +317,20 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
 
 template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
 __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks,
-                                                                unsigned period) {
-  // Every period-th block owns pages, the others rotate q: the former wait for one load after another, the latter for
-  // bandwidth, so they fill each other's gaps (17438 tokens: 132 us with the page blocks first, 122 us mixed).  With a
-  // token a sequence the pages take longest and go first (period 1; 250 sequences: 6.3 us, mixed 7.2).  Four blocks an SM
-  // (64 registers, a few spilled in the page part) hide more of the waiting than three: 125 us.
-  const unsigned turn = blockIdx.x / period;
-  if (turn < page_blocks && blockIdx.x == turn * period) {
+                                                                unsigned mix) {
+  // Blocks that own pages are spread evenly among those that rotate q: the former wait for one load after another, the
+  // latter for bandwidth, so they fill each other's gaps (17438 tokens: 132 us with the page blocks first, 115 us mixed).
+  // With a token a sequence the pages take longest and go first (mix 0; 250 sequences: 6.3 us, mixed 7.2).  Four blocks an
+  // SM (64 registers, a few spilled in the page part) hide more of the waiting than three.
+  // mix is page_blocks / blocks in 32 fraction bits, rounded up: i * mix passes each whole number below page_blocks once.
+  const unsigned i = blockIdx.x;
+  const unsigned before = mix ? __umulhi(i, mix) : min(i, page_blocks);  // page blocks in front of this one
+  if (mix ? __umulhi(i + 1, mix) > before : i < page_blocks) {
     constexpr int kPerBlock = kThreads / kGroup;
-    const long long work = static_cast<long long>(turn) * kPerBlock + threadIdx.x / kGroup;
+    const long long work = static_cast<long long>(before) * kPerBlock + threadIdx.x / kGroup;
     if (work < works) append_page<T, kInterleaved, kGroup, kHold>(p, work);
   } else {
-    rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(blockIdx.x - min(page_blocks, turn + 1)));
+    rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(i - before));
   }
 }
 
@@ -341,10 +343,10 @@ cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
   const long long q_blocks = (items + kThreads - 1) / kThreads;
   if (page_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (page_blocks + q_blocks == 0) return cudaSuccess;
+  const long long blocks = page_blocks + q_blocks;
+  const unsigned mix = kHold > 1 && q_blocks > 0 ? static_cast<unsigned>(((page_blocks << 32) + blocks - 1) / blocks) : 0u;
   kv_append_kernel<T, kInterleaved, kGroup, kHold, kHeads>
-      <<<static_cast<unsigned>(page_blocks + q_blocks), kThreads, 0, stream>>>(
-          p, works, static_cast<unsigned>(page_blocks),
-          static_cast<unsigned>(kHold > 1 && page_blocks > 0 ? (page_blocks + q_blocks) / page_blocks : 1));
+      <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p, works, static_cast<unsigned>(page_blocks), mix);
   return cudaGetLastError();
 }
 
