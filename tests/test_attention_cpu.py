@@ -54,7 +54,8 @@ def test_append_refuses_bad_arguments(cdll, ptr):
                dict(rows=_rows(ptr, batch=-1)), dict(rows=_rows(0)), dict(cache=_cache(0)), dict(cache=_cache(ptr, heads=0)),
                dict(rows=_rows(ptr, batch=0, tokens=3, cu=ptr))):
         assert call(**kw) == lib.BAD_ARG, kw
-    for kw in (dict(q=ptr + 2), dict(k=ptr + 8), dict(q_token=252), dict(k_token=130), dict(rot=24), dict(table=ptr + 4),
+    two = _rows(ptr, batch=2, tokens=2)  # (a pitch that is never used may be odd)
+    for kw in (dict(q=ptr + 2), dict(k=ptr + 8), dict(q_token=252, rows=two), dict(k_token=130, rows=two), dict(rot=24), dict(table=ptr + 4),
                dict(cache=_cache(ptr, dim=96)), dict(cache=_cache(ptr, size=24)), dict(cache=_cache(ptr, pitch=(2048, 1024, 72)))):
         assert call(**kw) == lib.UNSUPPORTED_ALIGNMENT, kw
     assert call(rows=_rows(ptr, batch=1 << 30, tokens=1 << 30)) == lib.TOO_LARGE
@@ -69,7 +70,8 @@ def test_attention_refuses_bad_arguments(cdll, ptr):
     for kw in (dict(q=None), dict(out=None), dict(dtype=2), dict(heads=5), dict(cache=None), dict(rows=None),
                dict(rows=_rows(ptr, tokens=2)), dict(rows=_rows(0))):
         assert call(**kw) == lib.BAD_ARG, kw
-    for kw in (dict(q=ptr + 8), dict(out=ptr + 4), dict(q_token=260), dict(o_token=258), dict(ws=ptr + 8),
+    two = _rows(ptr, batch=2, tokens=2)
+    for kw in (dict(q=ptr + 8), dict(out=ptr + 4), dict(q_token=260, rows=two), dict(o_token=258, rows=two), dict(ws=ptr + 8),
                dict(cache=_cache(ptr, dim=32)), dict(cache=_cache(ptr, size=256))):
         assert call(**kw) == lib.UNSUPPORTED_ALIGNMENT, kw
     assert call(rows=_rows(ptr, batch=0, tokens=0)) == lib.OK

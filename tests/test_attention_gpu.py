@@ -163,7 +163,7 @@ def test_rotary_edges(cuda_device):
     assert ops.rotary(x[:0], pos[:0], table).shape == (0, 2, 96)
     bad = [dict(x=x.int()), dict(x=x[0]), dict(x=x.transpose(1, 2)), dict(positions=pos[:4]), dict(positions=pos.float()),
            dict(table=table.double()), dict(table=table[:, :63]), dict(table=_table(16, 128)), dict(positions=pos.cpu()),
-           dict(out=x.float()), dict(out=x[:4])]
+           dict(out=x.float()), dict(out=x[:4]), dict(out=x[:1].expand(5, 2, 96))]
     for kw in bad:
         with pytest.raises(ValueError):
             ops.rotary(**{**dict(x=x, positions=pos, table=table), **kw})
@@ -440,6 +440,21 @@ def test_append_skips_what_is_not_there(cuda_device):
     _check_append(case, q, k, v, _table(256, 64), q_out=q)
 
 
+def test_pitches_that_are_never_used_may_be_odd(cuda_device):
+    """One token, one kv head, one page: their strides lead nowhere and need no alignment."""
+    from tritonbench_b200 import ops
+
+    codes = torch.zeros(2, 16 * 64 + 8, dtype=torch.uint8, device="cuda")[1:, 8 : 8 + 16 * 64]  # rows of 1032 bytes
+    k, v = (codes.clone().as_strided((1, 1, 16, 64), (1033, 1031, 64, 1)).view(E4M3) for _ in range(2))
+    scales = [torch.zeros(1, 1, device="cuda") for _ in range(2)]
+    cache = ops.Fp8KvCache(k, v, *scales)
+    one = torch.randn(1, 1, 64, device="cuda").bfloat16()
+    x = one.as_strided((1, 1, 64), (67, 65, 1))
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.fp8_kv_append(x, x, x, cache, table, lens), one)
+    assert torch.equal(ops.fp8_kv_attention(x, cache, table, lens).float(), (v[0, 0, 0].float() * scales[1]).bfloat16().float()[None])
+
+
 def test_append_without_q_and_without_tokens(cuda_device):
     from tritonbench_b200 import ops
 
@@ -464,7 +479,7 @@ def test_append_refuses(cuda_device):
                dict(k=k[..., :32], v=v[..., :32]), dict(cu_seqlens=None), dict(cu_seqlens=case.cu[:2]), dict(cu_seqlens=case.cu.long()),
                dict(seq_lens=case.seq_lens.long()), dict(seq_lens=case.seq_lens[:1]), dict(block_table=case.block_table.long()),
                dict(block_table=case.block_table.cpu()), dict(table=table.half()), dict(table=_table(8, 128)), dict(table=table.cpu()),
-               dict(q_out=q.float()), dict(q=None, q_out=q), dict(cache=None), dict(q=q.cpu())):
+               dict(q_out=q.float()), dict(q_out=q[:1].expand(5, 4, 64)), dict(q=None, q_out=q), dict(cache=None), dict(q=q.cpu())):
         with pytest.raises(ValueError):
             ops.fp8_kv_append(**{**good, **kw})
     odd = torch.zeros(5, 4 * 64 + 4, device="cuda", dtype=BF16)[:, 4:].unflatten(1, (4, 64))
@@ -778,7 +793,7 @@ def test_attention_refuses(cuda_device):
     good = dict(q=q, cache=case.cache, block_table=case.block_table, seq_lens=case.seq_lens, cu_seqlens=case.cu)
     for kw in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[0]), dict(cu_seqlens=None), dict(cu_seqlens=case.cu[:2]),
                dict(seq_lens=case.seq_lens.long()), dict(block_table=case.block_table[0]), dict(block_table=case.block_table[:1]),
-               dict(out=q.half()), dict(out=q[:3]), dict(q=q.cpu()), dict(cache=(1, 2)), dict(seq_lens=case.seq_lens.cpu())):
+               dict(out=q.half()), dict(out=q[:3]), dict(out=q[:, :1].expand(5, 4, 64)), dict(q=q.cpu()), dict(cache=(1, 2)), dict(seq_lens=case.seq_lens.cpu())):
         with pytest.raises(ValueError):
             ops.fp8_kv_attention(**{**good, **kw})
     odd = torch.zeros(5, 4 * 64 + 4, device="cuda", dtype=BF16)[:, 4:].unflatten(1, (4, 64))

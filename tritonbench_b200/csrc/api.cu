@@ -916,6 +916,9 @@ int b200fp8_rotary(const void* x, int dtype, void* y, int64_t tokens, int64_t he
 
 namespace {
 
+// a pitch that is used (more than one step of it) and is not a multiple of `unit`
+bool uneven(int64_t count, int64_t pitch, int64_t unit) { return count > 1 && pitch % unit != 0; }
+
 // what both calls on a paged cache ask of its descriptor and of the batch
 int check_kv(const b200fp8_kv_cache* c, const b200fp8_kv_batch* r, int64_t heads) {
   if (c == nullptr || r == nullptr) return B200FP8_BAD_ARG;
@@ -934,7 +937,8 @@ int check_kv(const b200fp8_kv_cache* c, const b200fp8_kv_batch* r, int64_t heads
   }
   if (!aligned16(c->k) || !aligned16(c->v)) return B200FP8_UNSUPPORTED_ALIGNMENT;
   for (int i = 0; i < 3; ++i) {
-    if (c->k_pitch[i] % 16 != 0 || c->v_pitch[i] % 16 != 0) return B200FP8_UNSUPPORTED_ALIGNMENT;
+    const int64_t count = i == 0 ? c->num_pages : (i == 1 ? c->kv_heads : c->page_size);
+    if (uneven(count, c->k_pitch[i], 16) || uneven(count, c->v_pitch[i], 16)) return B200FP8_UNSUPPORTED_ALIGNMENT;
     const int64_t most = i == 2 ? 0x7FFFFFFFll / c->page_size : 0x7FFFFFFFll;  // offsets inside a page fit 32 bits
     if (c->k_pitch[i] < 0 || c->v_pitch[i] < 0 || c->k_pitch[i] > most || c->v_pitch[i] > most) return B200FP8_TOO_LARGE;
   }
@@ -998,8 +1002,11 @@ int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, 
   if (rows->tokens == 0) return B200FP8_OK;
   if (k == nullptr || v == nullptr || (q != nullptr && q_out == nullptr)) return B200FP8_BAD_ARG;
   if (table != nullptr && (rot % 16 != 0 || !aligned16(table))) return B200FP8_UNSUPPORTED_ALIGNMENT;
-  if (!aligned16(k) || !aligned16(v) || (k_token | k_head | v_token | v_head) % 8 != 0) return B200FP8_UNSUPPORTED_ALIGNMENT;
-  if (q != nullptr && (!aligned16(q) || !aligned16(q_out) || (q_token | q_head | qo_token | qo_head) % 8 != 0)) {
+  const int64_t kv = cache->kv_heads, tokens = rows->tokens;
+  if (!aligned16(k) || !aligned16(v) || uneven(tokens, k_token | v_token, 8) || uneven(kv, k_head | v_head, 8)) {
+    return B200FP8_UNSUPPORTED_ALIGNMENT;
+  }
+  if (q != nullptr && (!aligned16(q) || !aligned16(q_out) || uneven(tokens, q_token | qo_token, 8) || uneven(heads, q_head | qo_head, 8))) {
     return B200FP8_UNSUPPORTED_ALIGNMENT;
   }
   KvAppendParams p = {};
@@ -1066,8 +1073,8 @@ int b200fp8_kv_attention(const void* q, void* out, float* lse, int dtype, int64_
   if (dtype != kQuantBf16 && dtype != kQuantFp16) return B200FP8_BAD_ARG;
   if (rows->tokens == 0) return B200FP8_OK;
   if (q == nullptr || out == nullptr) return B200FP8_BAD_ARG;
-  if (!aligned16(q) || (q_token | q_head) % 8 != 0 || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
-      (o_token | o_head) % 4 != 0 || !aligned16(workspace)) {
+  if (!aligned16(q) || uneven(rows->tokens, q_token, 8) || uneven(heads, q_head, 8) || (reinterpret_cast<uintptr_t>(out) & 7u) != 0 ||
+      uneven(rows->tokens, o_token, 4) || uneven(heads, o_head, 4) || !aligned16(workspace)) {
     return B200FP8_UNSUPPORTED_ALIGNMENT;
   }
   KvAttentionParams p = kv_attention_params(*cache, *rows, heads);

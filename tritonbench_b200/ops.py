@@ -350,6 +350,13 @@ def _fresh_like(x: torch.Tensor) -> torch.Tensor:
     return out if out.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _check_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device() or out.stride(2) != 1:
+        raise ValueError(f"{name} must have the input's shape, dtype and device, the last dimension contiguous")
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{name} must not be expanded: several of its elements are one")
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, table, interleaved, transpose):
@@ -404,8 +411,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
         return _Rotary.apply(x, positions, table, interleaved, transpose)
     if out is None:
         out = _fresh_like(x)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.get_device() != device or out.stride(2) != 1:
-        raise ValueError("out must have x's shape, dtype and device, dim contiguous")
+    else:
+        _check_out(out, x, "out")
     if tokens == 0 or heads == 0:
         return out
     if device != torch.cuda.current_device():  # a launch on a stream of another device is an error
@@ -422,9 +429,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
 
 class Fp8KvCache:
     """A paged key/value cache in e4m3: k and v [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn (any page, head
-    and row strides that are multiples of 16 and below 2^31; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads] float32;
-    a value is code * scale, no scale is negative.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object describes the four tensors
-    and keeps them alive; make one with `empty`, or around tensors of your own."""
+    and row strides that are multiples of 16 and below 2^31; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads]
+    float32; a value is code * scale, no scale is negative.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object
+    describes the four tensors and keeps them alive; make one with `empty`, or around tensors of your own."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor")
 
@@ -446,7 +453,7 @@ class Fp8KvCache:
         if k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("head_dim must be contiguous in k and v")
         for t in (k, v):
-            if t.data_ptr() % 16 or any(st % 16 for st in t.stride()[:3]):
+            if t.data_ptr() % 16 or any(st % 16 for st, n in zip(t.stride()[:3], t.shape) if n > 1):
                 raise NotImplementedError("rows of k and v must start on 16-byte boundaries")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
@@ -539,8 +546,8 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
             raise ValueError("q must have head_dim contiguous")
         if q_out is None:
             q_out, fill = _fresh_like(q), 1
-        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != device or q_out.stride(2) != 1:
-            raise ValueError("q_out must have q's shape, dtype and device, head_dim contiguous")
+        else:
+            _check_out(q_out, q, "q_out")
         o_token, o_head, _ = q_out.stride()
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -579,7 +586,8 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows behind
     cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for up to a few dozen new
     tokens a sequence: the cache is read once per 16 query rows, with the work split over the context.  The result does
-    not depend on timing.  The workspace is allocated per call, so captured graphs and streams never share one."""
+    not depend on timing.  Small calls need no workspace, the others allocate theirs, so captured graphs and streams never
+    share one."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
     device = cache.device
@@ -599,8 +607,8 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     fill = 0
     if out is None:
         out, fill = _fresh_like(q), 1
-    elif out.shape != q.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
-        raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+    else:
+        _check_out(out, q, "out")
     o_token, o_head, _ = out.stride()
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
