@@ -95,6 +95,18 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// lo += low half of h, hi += its high half, rounded once in fp32
+__device__ __forceinline__ void add_halves(float& lo, float& hi, uint32_t h) {
+  asm("{\n"
+      ".reg .f16 a, b, one;\n"
+      "mov.b32 {a, b}, %2;\n"
+      "mov.b16 one, 0x3c00;\n"
+      "fma.rn.f32.f16 %0, a, one, %0;\n"
+      "fma.rn.f32.f16 %1, b, one, %1;\n"
+      "}\n"
+      : "+f"(lo), "+f"(hi)
+      : "r"(h));
+}
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -726,8 +738,8 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
       }
       // V scales: O is kept in units of the chunk's largest one, so that products can be added to it where they are; p is
-      // multiplied by what a page's scale is of that, which stays exact enough in fp16 down to an eighth.  (Scales that
-      // are powers of two are mostly alike.)
+      // multiplied by what a page's scale is of that, down to an eighth: exact for scales that are powers of two (which are
+      // mostly alike), else two more roundings to fp16.
       float v_max = 0.0f;
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) v_max = there[sub] ? fmaxf(v_max, v_scale[sub]) : v_max;
@@ -741,11 +753,14 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
       }
       mixed = mixed && plain;
-      float share[S::kSubs];
+      uint32_t share[S::kSubs];  // of the largest scale, twice in fp16
       if (S::kSubs > 1 && mixed) {
         const float inv = 1.0f / v_max;
 #pragma unroll
-        for (int sub = 0; sub < S::kSubs; ++sub) share[sub] = there[sub] ? v_scale[sub] * inv : 1.0f;
+        for (int sub = 0; sub < S::kSubs; ++sub) {
+          const float f = there[sub] ? v_scale[sub] * inv : 1.0f;
+          share[sub] = half2_of(f, f);
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
@@ -756,20 +771,22 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
           const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
           const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
           const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
-          l[nt][0] += p0 + p2;
-          l[nt][1] += p1 + p3;
-          s[mt][nt][0] = p0, s[mt][nt][1] = p1, s[mt][nt][2] = p2, s[mt][nt][3] = p3;
+          // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient
+          pf[mt][nt][0] = half2_of(p0, p1);
+          pf[mt][nt][1] = half2_of(p2, p3);
+          add_halves(l[nt][0], l[nt][1], pf[mt][nt][0]);
+          add_halves(l[nt][0], l[nt][1], pf[mt][nt][1]);
         }
         if (S::kSubs > 1 && mixed) {
 #pragma unroll
           for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][nt][e] *= share[mt * 16 / kSub];
+            for (int i = 0; i < 2; ++i) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(pf[mt][nt][i]) : "r"(share[mt * 16 / kSub]));
         }
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
-          pf[mt][nt][0] = transpose8x8(half2_of(s[mt][nt][0], s[mt][nt][1]));
-          pf[mt][nt][1] = transpose8x8(half2_of(s[mt][nt][2], s[mt][nt][3]));
+          pf[mt][nt][0] = transpose8x8(pf[mt][nt][0]);
+          pf[mt][nt][1] = transpose8x8(pf[mt][nt][1]);
         }
       }
       bool strange = false;
