@@ -49,18 +49,14 @@ constexpr uint32_t kNoPage = 0xffffffffu;  // in place of a chunk's k_scale: its
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-template <int kBytes, bool kAlways = true>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take = true) {  // zeros where not taken
-  const int n = take ? kBytes : 0;
-  if constexpr (kBytes == 16 && kAlways) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  } else if constexpr (kBytes == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  } else if constexpr (kAlways) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(n) : "memory");
-  }
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool take) {  // zeros where not taken
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -509,10 +505,14 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
             for (int n = 0; n < kSub / kCopyRows; ++n) {
               const int row = sub * kSub + n * kCopyRows;
               const uint32_t to = base + copy_at[n % kPlaces] + row / 8 * k8Rows;
-              const bool take = whole.value || n * kCopyRows + copy_row < left;
-              // (q: an address that is not read, and there even when the cache has no page)
-              copy_async<16, whole.value>(to, take ? static_cast<const void*>(k + n * kCopyRows * k_row) : p.q, take);
-              copy_async<16, whole.value>(to + S::kTileBytes, take ? static_cast<const void*>(v + n * kCopyRows * v_row) : p.q, take);
+              if constexpr (whole.value) {
+                copy_async16(to, k + n * kCopyRows * k_row);
+                copy_async16(to + S::kTileBytes, v + n * kCopyRows * v_row);
+              } else {  // (q: an address that is not read, and there even when the cache has no page)
+                const bool take = n * kCopyRows + copy_row < left;
+                copy_async16(to, take ? static_cast<const void*>(k + n * kCopyRows * k_row) : p.q, take);
+                copy_async16(to + S::kTileBytes, take ? static_cast<const void*>(v + n * kCopyRows * v_row) : p.q, take);
+              }
             }
           }
         };
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
           if (page < 0) {
             *reinterpret_cast<uint32_t*>(at + 2 * S::kTileBytes + 4 * lane) = kNoPage;
           } else {
-            copy_async<4>(base + 2 * S::kTileBytes + 4 * lane,
+            copy_async4(base + 2 * S::kTileBytes + 4 * lane,
                           (lane & 1) ? p.v_scale + static_cast<long long>(page) * p.vs_page + static_cast<long long>(ahead.kv_head) * p.vs_head
                                      : p.k_scale + static_cast<long long>(page) * p.ks_page + static_cast<long long>(ahead.kv_head) * p.ks_head);
           }
