@@ -15,7 +15,7 @@
 // Bound by HBM for prompts (q in, q out, k and v in at 2 bytes, out at 1), by latency for single tokens.  One launch
 // does it all.  Some blocks own pages: each group of threads has one (page, kv head, k or v), so that nothing but that
 // group reads or writes the page's scale: no atomics and the same result every time.  The other blocks rotate q.  A
-// group is a warp when a sequence brings about one token or a page is small, else a block; its rows stay in registers
+// group is a warp when a sequence brings a few tokens or a page is small, else a block; its rows stay in registers
 // between the maximum and the codes.
 #include <cuda_fp8.h>
 
@@ -352,9 +352,12 @@ cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
 
 template <typename T, bool kInterleaved>
 cudaError_t launch_i(const KvAppendParams& p, cudaStream_t stream) {
-  // about one token a sequence: a block for every page would leave nearly all of its threads idle
-  if (p.cu_seqlens == nullptr || p.tokens <= 2ll * p.batch) return launch_t<T, kInterleaved, 32, 1, 1>(p, stream);
-  // two slots a thread: a warp for 16 tokens of 64, a block for 64 tokens of 128
+  // A few tokens a sequence: a block for every page would leave nearly all of its threads idle.  Device us, warp / block a
+  // page, 8 kv heads of 128: 250 sequences x 1 token 6.3 / 18.6; 64 x 6 7.0 / 11.5, x 12 10.3 / 13.5, x 48 33 / 30;
+  // 8 x 6 4.8 / 4.6, x 24 9.7 / 5.0.
+  if (p.tokens <= 8ll * p.batch) return launch_t<T, kInterleaved, 32, 1, 1>(p, stream);
+  // Two slots a thread: a warp for 16 tokens of 64 (5000 tokens in such pages 16.5 us, a block each 31.2), a block for 64
+  // tokens of 128 (17438 tokens 115 us, a warp each 172).
   if (p.page_size * (p.dim / (2 * kN)) <= 64) return launch_t<T, kInterleaved, 32, 2, 4>(p, stream);
   return launch_t<T, kInterleaved, kThreads, 2, 4>(p, stream);
 }

@@ -128,7 +128,8 @@ cudaError_t launch_any(const RotaryParams& p, cudaStream_t stream) {
   constexpr int kN = 16 / sizeof(T);
   const bool vector = p.vector_ok && (p.rot / 2) % kN == 0 && p.dim % kN == 0;
   if (!vector) return launch_t<T, 1, 1>(p, stream);
-  // few tokens: more threads rather than more loads a thread
+  // Few tokens: more threads rather than more loads a thread.  Device us with four heads a thread / one, 40 heads of 128:
+  // 64 tokens 2.7 / 2.1, 256 2.7 / 2.6, 512 3.5 / 3.6, 2048 6.6 / 8.1, 8192 30.2 / 32.7.
   const long long threads = static_cast<long long>(p.tokens) * p.heads * (p.dim / (2 * kN));
   if (threads >= kManyThreads) return launch_t<T, kN, 4>(p, stream);
   return launch_t<T, kN, 1>(p, stream);
