@@ -370,6 +370,16 @@ def test_append_to_other_layouts(cuda_device, layout, kv, group):
     assert torch.equal(q._base, before)
 
 
+@pytest.mark.parametrize("dim,page,dtype", [(128, 64, BF16), (256, 32, FP16), (64, 128, BF16), (64, 16, FP16)])
+@pytest.mark.parametrize("new", [[1] * 40 + [400] + [1] * 23, [50, 1, 0, 2] * 20, [1, 17, 16, 15] * 16, [6] * 64])
+def test_append_of_few_and_many_tokens_in_one_batch(cuda_device, new, dim, page, dtype):
+    """Prompts among sequences of a token or a few: pages that get a few rows lie beside pages that get all of theirs."""
+    case = Case([n + (7 * i) % 150 for i, n in enumerate(new)], new, kv=8, group=1, dim=dim, page=page, dtype=dtype, seed=dim)
+    q, k, v = (t.clone() for t in _qkv(case))
+    k[len(k) // 2, :, 3], v[-1, 1, 0], v[45:60, 2] = float("inf"), float("nan"), float("-inf")
+    _check_append(case, q, k, v, _table(1024, 64))
+
+
 def test_appended_page_grows_its_scale_step_by_step(cuda_device):
     """Tokens of growing size into one page: every growth moves the codes that are there, exactly but for subnormals."""
     lens = [1]

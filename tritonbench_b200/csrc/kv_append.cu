@@ -15,8 +15,8 @@
 // Bound by HBM for prompts (q in, q out, k and v in at 2 bytes, out at 1), by latency for single tokens.  One launch
 // does it all.  Some blocks own pages: each group of threads has one (page, kv head, k or v), so that nothing but that
 // group reads or writes the page's scale: no atomics and the same result every time.  The other blocks rotate q.  A
-// group is a warp when a sequence brings a few tokens or a page is small, else a block; its rows stay in registers
-// between the maximum and the codes.
+// group is a warp when few rows come to a page or it is small, else a block; its rows stay in registers between the
+// maximum and the codes.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -102,13 +102,17 @@ __device__ __forceinline__ void turn(const KvAppendParams& p, long long pos, int
   rotate_slot<kN, kInterleaved>(a, b, c, s);
 }
 
-// One page, one kv head, k or v.  kGroup threads: a warp or the block.
-template <typename T, bool kInterleaved, int kGroup, int kHold>
-__device__ __forceinline__ void append_page(const KvAppendParams& p, long long work) {
-  const int in_group = static_cast<int>(threadIdx.x) % kGroup;
-  const int which = static_cast<int>(work & 1);
+// One page, one kv head, k or v: the rows that come to it.
+struct PageRows {
+  int which, head, page, held, rows;
+  long long from, token0;  // position and token of the first row
+};
+
+// false: no row comes to this one
+__device__ __forceinline__ bool find_rows(const KvAppendParams& p, long long work, PageRows& w) {
+  w.which = static_cast<int>(work & 1);
   const long long rest = work >> 1;
-  const int head = static_cast<int>(rest % p.kv_heads);
+  w.head = static_cast<int>(rest % p.kv_heads);
   const long long slot_no = rest / p.kv_heads;
   // slot_no -> sequence and page: sequence b owns the slots from cu[b] / page_size + 2 b on, at least as many as the
   // pages that its tokens can touch
@@ -128,18 +132,27 @@ __device__ __forceinline__ void append_page(const KvAppendParams& p, long long w
   }
   const long long end = p.seq_lens[b];          // positions [begin, end) of the sequence are new
   const long long begin = end - count;          // negative: more tokens than the sequence has; those are left out
-  if (count <= 0 || page_no < 0) return;
+  if (count <= 0 || page_no < 0) return false;
   page_no += (begin > 0 ? begin : 0) >> p.page_shift;
-  if (page_no >= p.table_width) return;
+  if (page_no >= p.table_width) return false;
   const long long lo = page_no << p.page_shift;
-  const long long from = lo > begin ? lo : begin;
+  w.from = lo > begin ? lo : begin;
   const long long to = lo + p.page_size < end ? lo + p.page_size : end;
-  if (from >= to) return;
-  const long long token0 = first_token + (from - begin);
-  const int rows = static_cast<int>(to - from);
-  if (token0 < 0 || token0 + rows > p.tokens) return;  // lengths that do not belong to this q, k, v
-  const int held = static_cast<int>(from - lo);
-  const int page = p.block_table[b * p.bt_stride + page_no];  // on its way while the rows are read
+  if (w.from >= to) return false;
+  w.token0 = first_token + (w.from - begin);
+  w.rows = static_cast<int>(to - w.from);
+  if (w.token0 < 0 || w.token0 + w.rows > p.tokens) return false;  // lengths that do not belong to this q, k, v
+  w.held = static_cast<int>(w.from - lo);
+  w.page = p.block_table[b * p.bt_stride + page_no];  // on its way while the rows are read
+  return true;
+}
+
+// kGroup threads: a warp or the block
+template <typename T, bool kInterleaved, int kGroup, int kHold>
+__device__ __forceinline__ void append_rows(const KvAppendParams& p, const PageRows& w) {
+  const int in_group = static_cast<int>(threadIdx.x) % kGroup;
+  const int which = w.which, head = w.head, page = w.page, held = w.held, rows = w.rows;
+  const long long from = w.from, token0 = w.token0;
   const T* x = which ? static_cast<const T*>(p.v) + token0 * p.v_token + head * p.v_head
                      : static_cast<const T*>(p.k) + token0 * p.k_token + head * p.k_head;
   const long long x_token = which ? p.v_token : p.k_token;
@@ -315,7 +328,13 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
   }
 }
 
-template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
+// Who appends: a warp a page, a block a page, or a warp each for pages that get a few rows and the block for the others.
+enum { kWarps, kBlock, kEither };
+// Rows x slots up to which a warp does a page by itself in kEither: 16 rows of 128 (64 sequences x 12 tokens 10.7 us, with a
+// limit of 64 22.6; 63 x 1 and one of 400 the same with 32 to 192).
+constexpr int kWarpItems = 128;
+
+template <typename T, bool kInterleaved, int kWho, int kHold, int kHeads>
 __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const KvAppendParams p, long long works, unsigned page_blocks,
                                                                 unsigned mix) {
   // Blocks that own pages are spread evenly among those that rotate q: the former wait for one load after another, the
@@ -326,40 +345,68 @@ __global__ void __launch_bounds__(kThreads, 4) kv_append_kernel(const KvAppendPa
   const unsigned i = blockIdx.x;
   const unsigned before = mix ? __umulhi(i, mix) : min(i, page_blocks);  // page blocks in front of this one
   if (mix ? __umulhi(i + 1, mix) > before : i < page_blocks) {
-    constexpr int kPerBlock = kThreads / kGroup;
-    const long long work = static_cast<long long>(before) * kPerBlock + threadIdx.x / kGroup;
-    if (work < works) append_page<T, kInterleaved, kGroup, kHold>(p, work);
+    PageRows w;
+    if constexpr (kWho == kBlock) {
+      if (find_rows(p, before, w)) append_rows<T, kInterleaved, kThreads, kHold>(p, w);
+    } else if constexpr (kWho == kWarps) {
+      const long long work = static_cast<long long>(before) * (kThreads / 32) + threadIdx.x / 32;
+      if (work < works && find_rows(p, work, w)) append_rows<T, kInterleaved, 32, kHold>(p, w);
+    } else {
+      // a page's heads and a prompt's pages lie in different blocks, so that no block gets many that are large
+      const auto work_of = [&](int warp) { return before + static_cast<long long>(page_blocks) * warp; };
+      __shared__ bool large[kThreads / 32];
+      const int warp = static_cast<int>(threadIdx.x / 32);
+      const bool found = work_of(warp) < works && find_rows(p, work_of(warp), w);
+      const bool by_warp = found && w.rows * (p.dim / (2 * kN)) <= kWarpItems;
+      if (threadIdx.x % 32 == 0) large[warp] = found && !by_warp;
+      const bool any = __syncthreads_or(found && !by_warp);
+      if (by_warp) append_rows<T, kInterleaved, 32, kHold>(p, w);
+      if (!any) return;
+      for (int i = 0; i < kThreads / 32; ++i) {
+        if (large[i] && find_rows(p, work_of(i), w)) append_rows<T, kInterleaved, kThreads, kHold>(p, w);
+      }
+    }
   } else {
     rotate_q<T, kInterleaved, kHeads>(p, static_cast<long long>(i - before));
   }
 }
 
-template <typename T, bool kInterleaved, int kGroup, int kHold, int kHeads>
-cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
+// (page, kv head, k or v) that tokens may come to
+long long works_of(const KvAppendParams& p) {
   const long long page_slots = p.cu_seqlens == nullptr ? p.batch : (p.tokens >> p.page_shift) + 2ll * p.batch;
-  const long long works = page_slots * p.kv_heads * 2;
-  const long long page_blocks = (works + kThreads / kGroup - 1) / (kThreads / kGroup);
+  return page_slots * p.kv_heads * 2;
+}
+
+template <typename T, bool kInterleaved, int kWho, int kHold, int kHeads>
+cudaError_t launch_t(const KvAppendParams& p, cudaStream_t stream) {
+  const long long works = works_of(p);
+  constexpr int kPerBlock = kWho == kBlock ? 1 : kThreads / 32;
+  const long long page_blocks = (works + kPerBlock - 1) / kPerBlock;
   const long long items = p.q == nullptr ? 0 : static_cast<long long>(p.tokens) * ((p.heads + kHeads - 1) / kHeads) * (p.dim / (2 * kN));
   const long long q_blocks = (items + kThreads - 1) / kThreads;
   if (page_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (page_blocks + q_blocks == 0) return cudaSuccess;
   const long long blocks = page_blocks + q_blocks;
   const unsigned mix = kHold > 1 && q_blocks > 0 ? static_cast<unsigned>(((page_blocks << 32) + blocks - 1) / blocks) : 0u;
-  kv_append_kernel<T, kInterleaved, kGroup, kHold, kHeads>
+  kv_append_kernel<T, kInterleaved, kWho, kHold, kHeads>
       <<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p, works, static_cast<unsigned>(page_blocks), mix);
   return cudaGetLastError();
 }
 
 template <typename T, bool kInterleaved>
 cudaError_t launch_i(const KvAppendParams& p, cudaStream_t stream) {
-  // A few tokens a sequence: a block for every page would leave nearly all of its threads idle.  Device us, warp / block a
-  // page, 8 kv heads of 128: 250 sequences x 1 token 6.3 / 18.6; 64 x 6 7.0 / 11.5, x 12 10.3 / 13.5, x 48 33 / 30;
-  // 8 x 6 4.8 / 4.6, x 24 9.7 / 5.0.
-  if (p.tokens <= 8ll * p.batch) return launch_t<T, kInterleaved, 32, 1, 1>(p, stream);
+  // One token a sequence: a block for every page would leave nearly all of its threads idle.  Device us, warp / block a
+  // page, 8 kv heads of 128: 250 sequences 6.3 / 18.6.
+  if (p.cu_seqlens == nullptr) return launch_t<T, kInterleaved, kWarps, 1, 1>(p, stream);
+  // More pages than a wave of blocks (148 SMs x 4) and few tokens a sequence, or a prompt among many single tokens.  Device
+  // us, this / a block a page / a warp a page: 64 sequences x 1 token 4.4 / 9.5 / 4.1, x 12 10.2 / 13.1 / 10.0, x 16 12.7 /
+  // 15.1, x 24 26.1 / 17.5 / 17.1; 63 x 1 and one of 400 9.3 / 12.9 / 22.6; 250 x 1 and one of 1500 24.5 / 38.7 / 33.6.
+  // Fewer pages: 16 x 12 6.6 / 5.4, 8 x 6 5.1 / 4.5 / 4.9.
+  if (works_of(p) > 592 && p.tokens <= 16ll * p.batch) return launch_t<T, kInterleaved, kEither, 1, 1>(p, stream);
   // Two slots a thread: a warp for 16 tokens of 64 (5000 tokens in such pages 16.5 us, a block each 31.2), a block for 64
   // tokens of 128 (17438 tokens 115 us, a warp each 172).
-  if (p.page_size * (p.dim / (2 * kN)) <= 64) return launch_t<T, kInterleaved, 32, 2, 4>(p, stream);
-  return launch_t<T, kInterleaved, kThreads, 2, 4>(p, stream);
+  if (p.page_size * (p.dim / (2 * kN)) <= 64) return launch_t<T, kInterleaved, kWarps, 2, 4>(p, stream);
+  return launch_t<T, kInterleaved, kBlock, 2, 4>(p, stream);
 }
 
 template <typename T>
