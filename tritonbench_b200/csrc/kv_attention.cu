@@ -116,7 +116,8 @@ __device__ __forceinline__ bool has_nan_code(uint32_t w) {  // any byte 0x7f or 
 // ------------------------------------------------------------------ the list of units
 struct Seq {
   int n;          // new tokens
-  int len;        // context, the new tokens included
+  int begin;      // position of the first new token; negative: more of them than the sequence has tokens
+  int len;        // context, the new tokens included, as far as the block table goes
   int row_tiles;  // tiles of query rows
   int units;      // units of a tile, at least one (a tile without context still has an output)
   int q_base;     // first row of q
@@ -132,7 +133,9 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionParams& p, int b) {
   }
   s.q_base = first;
   s.n = last - first;
-  s.len = min(max(p.seq_lens[b], 0), p.max_len);
+  const int len = max(p.seq_lens[b], 0);
+  s.begin = len - s.n;
+  s.len = min(len, p.max_len);
   s.row_tiles = static_cast<int>((static_cast<long long>(s.n) * p.group + kRows - 1) / kRows);
   s.units = max((s.len + kUnit - 1) / kUnit, 1);
   return s;
@@ -172,13 +175,14 @@ struct Cursor {
   int kv_head, row0;
   int min_end, max_end;  // tokens that the tile's first and last query see: [0, end)
 
+  // new token i sees the tokens up to its own position that the block table has room for: [0, end_of(i))
+  __device__ __forceinline__ int end_of(int i) const { return min(max(s.begin + i + 1, 0), s.len); }
   __device__ __forceinline__ void enter_tile(const KvAttentionParams& p) {
     kv_head = tile / s.row_tiles;
     row0 = (tile - kv_head * s.row_tiles) * kRows;
     const int last_row = min(row0 + kRows, s.n * p.group) - 1;
-    const int begin = s.len - s.n;
-    min_end = max(begin + row0 / p.group + 1, 0);
-    max_end = max(begin + last_row / p.group + 1, 0);
+    min_end = end_of(row0 / p.group);
+    max_end = end_of(last_row / p.group);
   }
   __device__ __forceinline__ void enter_sequence(const KvAttentionParams& p) {
     s = seq_of<kRows, kUnit>(p, b);
@@ -584,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
       to[(2 * piece + 1) ^ (r & 1)] = make_uint4(h[4], h[5], h[6], h[7]);
       if (piece == 0) {
         row_scale[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (fabsf(p.softmax_scale) * kLog2e);
-        row_end[r] = r < rows ? cur.s.len - cur.s.n + token + 1 : 0;
+        row_end[r] = r < rows ? cur.end_of(token) : 0;
       }
     }
     __syncthreads();
