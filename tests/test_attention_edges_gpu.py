@@ -1,9 +1,18 @@
 """Edges of the rotary, cache-append and cache-attention calls, by the forms and bounds of test_attention_gpu.py."""
-import pytest
+import math
 
-from test_attention_gpu import BF16, FP16, Case, _check_append, _check_attention, _qkv
+import pytest
+import torch
+
+from test_attention_gpu import BF16, E4M3, FP16, TINY, Case, _check_append, _check_attention, _context, _half_step, _plain_attention, _qkv
 
 pytestmark = pytest.mark.gpu
+
+
+def _attention(case, q, **kw):
+    from tritonbench_b200 import ops
+
+    return ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens, case.cu, **kw)
 
 
 @pytest.mark.parametrize("dim,page,dtype", [(128, 16, BF16), (64, 64, FP16), (256, 32, BF16)])
@@ -20,3 +29,44 @@ def test_lengths_past_the_block_table_keep_their_positions(cuda_device, lens, ne
     q, k, v = _qkv(case, extra=1)
     rotated = _check_append(case, q, k, v)
     _check_attention(case, rotated)
+
+
+def _first_key_ahead(case, nats, share):
+    """q, and a cache whose sequence's first key scores `nats` above all others (which score zero) and has a zero value;
+    V scales that differ from page to page by up to `share`."""
+    q = torch.zeros(case.tokens, case.kv * case.group, case.dim, device="cuda")
+    q[..., 0] = nats / 8 * case.dim**0.5  # exact scores: one product
+    page = int(case.block_table[0, 0])
+    for t in (case.k, case.v):
+        t.view(torch.uint8)[page, :, 0] = 0
+    k = torch.zeros(case.k.shape, device="cuda")
+    k[page, :, 0, 0] = 8.0
+    case.k.view(torch.uint8).copy_(k.to(E4M3).view(torch.uint8))
+    case.ks.fill_(1.0)
+    case.vs.copy_(2.0**9 * torch.exp2(-torch.randint(0, int(math.log2(share)) + 1, case.vs.shape, generator=case.gen, device="cuda").float()))
+    return q.to(case.dtype)
+
+
+@pytest.mark.parametrize("dim,page,group", [(64, 16, 1), (64, 32, 9), (128, 16, 4), (128, 64, 12), (256, 16, 8)])
+@pytest.mark.parametrize("share", [1, 8])
+@pytest.mark.parametrize("nats", [14, 16, 17, 18, 20])
+def test_tokens_far_below_the_largest_score(cuda_device, nats, share, dim, page, group):
+    """A first token that takes nearly all of the weight and has nothing to give: what is left of the output comes from the
+    others, whose p is 2^-20 to 2^-29 of its.  p in fp16, the largest at least 2^11 of its units: below 2^-14 of them (2^-25
+    of the largest) it is off by 2^-25 of them, a weight by 2^-36, times 8 where a page's V scale is an eighth."""
+    case = Case([1500], None, kv=2, group=group, dim=dim, page=page, dtype=FP16)
+    case.v.view(torch.uint8).bitwise_and_(0x7F)  # magnitudes: the sum does not cancel
+    case.v.copy_(torch.where(case.v.float() == 0, 1.0, case.v.float()).to(E4M3))
+    q = _first_key_ahead(case, nats, share)
+    want, _, bound, _ = _plain_attention(case, q, dim**-0.5)
+    v, ok = _context(case, 0, case.v, case.vs)
+    assert bool(ok.all())
+    bound -= 2.0**-25 * v.abs().sum(0).repeat_interleave(group, 0)  # in place of the bound's absolute part
+    bound += 2.0**-36 * share * v.abs().sum(0).repeat_interleave(group, 0)
+    for wide in (False, True):
+        if wide:
+            case.widen()
+        got = _attention(case, q)
+        off = (got.double() - want).abs()
+        limit = bound + _half_step(FP16) * (want + bound) + TINY[FP16]
+        assert (off <= limit).all(), (float((off / want).max()), float((limit / want).max()))

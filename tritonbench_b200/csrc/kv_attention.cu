@@ -9,10 +9,11 @@
 //     that share a kv head - group heads x new tokens, mostly 4 to 8 - fill a tile of 8 columns, where they would fill
 //     half of a 16-row tile.  O^T = V^T P^T then has the head dimension as rows, and P^T goes from accumulator to
 //     operand layout with one movmatrix per 8 tokens.
-//   * e4m3 is exact in fp16, and so are bf16 queries once a row is scaled by a power of two (what falls below fp16's
-//     range then is under 2^-24 of the row's largest element); p rounded to fp16 is off by 2^-11 of itself at most.
-//     tcgen05 takes 8-bit operands only in pairs, which would round queries and p to 3 bits of mantissa.  Sums, maxima
-//     and the output stay in fp32.
+//   * e4m3 is exact in fp16, and so are queries once a row is scaled by a power of two, its largest element to [1, 2): of
+//     those that fp16 holds in fewer bits then (bf16 below 2^-17 of the row's largest, fp16 below 2^-14) an element is off by
+//     2^-25 of the largest at most.  p is rounded to fp16, to 2^-11 of itself, in units in which the largest is 2^11 to 2^15: what
+//     is below 2^-25 of it is off by up to 2^-36 of it.  tcgen05 takes 8-bit operands only in pairs, which would round
+//     queries and p to 3 bits of mantissa.  Sums, maxima and the output stay in fp32.
 //   * The order of the contraction is free, so a thread's operand elements are 16 neighbouring bytes of a token:
 //     whole 16-byte vectors are loaded, and the pairing of two tokens' V bytes costs one byte permute per 4 bytes.
 //     A warp copies (cp.async, whole rows) and reads its own chunks, so the ring needs no barrier beyond the warp.
@@ -89,6 +90,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// the same, and 65504 for what is larger
+__device__ __forceinline__ uint32_t finite_half2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 // lo += low half of h, hi += its high half, rounded once in fp32
@@ -663,10 +670,12 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
             for (int nt = 0; nt < kNT; ++nt) mma16816(s[mt][nt], a0, a1, a2, a3, qf[nt][2 * i], qf[nt][2 * i + 1]);
           }
       }
-      // ---- softmax over the tokens, column by column.  m is a reference that is at most kSlack below the largest score so
-      // far: O and l are rescaled only when a score passes it by more, which after a few chunks hardly happens (p is then
-      // at most 2^kSlack, well inside fp16, and its relative rounding is the same).
-      constexpr float kSlack = 8.0f;
+      // ---- softmax over the tokens, column by column.  The reference m is kBelow below a column's largest score when it is
+      // set, so that fp16's range lies where the weights are (without it, first tokens that take nearly all of the weight
+      // would leave the others, 17 and more below in units of e, to subnormals and zero).  It follows the largest score only
+      // when that has grown by more than kSlack: p is at most 2^(kBelow + kSlack), and O and l are hardly ever rescaled
+      // after a few chunks.
+      constexpr float kBelow = 11.0f, kSlack = 4.0f;
       uint32_t pf[S::kMT][kNT][2];
       // The factor of a page's scores goes into the exponent's argument (it is not negative, so the largest product is the
       // largest score); masked scores are multiplied first.
@@ -715,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
         top[nt][0] = top0 * (S::kSubs == 1 ? col[nt].x * k_scale[0] : col[nt].x);
         top[nt][1] = top1 * (S::kSubs == 1 ? col[nt].y * k_scale[0] : col[nt].y);
-        passed = passed || top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
+        passed = passed || top[nt][0] > m[nt][0] + (kBelow + kSlack) || top[nt][1] > m[nt][1] + (kBelow + kSlack);
       }
       if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
@@ -724,9 +733,10 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             f[c] = 1.0f;
-            if (top[nt][c] > m[nt][c] + kSlack) {
-              f[c] = exp2_approx(m[nt][c] - top[nt][c]);
-              m[nt][c] = top[nt][c];
+            if (top[nt][c] > m[nt][c] + (kBelow + kSlack)) {
+              const float to = top[nt][c] - kBelow;
+              f[c] = exp2_approx(m[nt][c] - to);
+              m[nt][c] = to;
               l[nt][c] *= f[c];
             }
           }
@@ -747,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
       float v_max = 0.0f;
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) v_max = there[sub] ? fmaxf(v_max, v_scale[sub]) : v_max;
-      bool plain = v_max <= kMaxFloat && v_max >= v_top * 0x1p-80f;
+      bool plain = v_max <= kMaxFloat && v_max >= v_top * 0x1p-72f;
       bool mixed = false;
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) {
@@ -775,9 +785,10 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
           const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
           const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
           const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
-          // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient
-          pf[mt][nt][0] = half2_of(p0, p1);
-          pf[mt][nt][1] = half2_of(p2, p3);
+          // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Scores of 2^23 and more are
+          // a unit off in fp32, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
+          pf[mt][nt][0] = finite_half2_of(p0, p1);
+          pf[mt][nt][1] = finite_half2_of(p2, p3);
           add_halves(l[nt][0], l[nt][1], pf[mt][nt][0]);
           add_halves(l[nt][0], l[nt][1], pf[mt][nt][1]);
         }
@@ -889,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
         product(std::false_type{}, 0, 0, 1.0f, [](int, int) { return true; });
       } else {
-        // Something that is not finite, or scales too far apart (zero, or 2^80 below the largest so far, would take O out
+        // Something that is not finite, or scales too far apart (zero, or 2^72 below the largest so far, would take O out
         // of fp32's range): every part on its own, added with its factor, once for every place where a column's context
         // can end in the part or behind it, with V cut there; columns that see nothing of the part take nothing from it.
         const int lo = min(max(cur.min_end - token0, 0), kChunk), hi = min(cur.max_end - token0, kChunk);
