@@ -70,3 +70,27 @@ def test_tokens_far_below_the_largest_score(cuda_device, nats, share, dim, page,
         off = (got.double() - want).abs()
         limit = bound + _half_step(FP16) * (want + bound) + TINY[FP16]
         assert (off <= limit).all(), (float((off / want).max()), float((limit / want).max()))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dim,page,group", [(64, 16, 1), (64, 32, 9), (128, 64, 12), (256, 16, 8)])
+@pytest.mark.parametrize("size", [2.0**20, 2.0**24, 2.0**28])
+def test_scores_that_fp32_holds_in_steps_of_several_units(cuda_device, size, dim, page, group, wide):
+    """Scores so large that the best of them is far from the next: its token's value is the output, whatever its p came to."""
+    case = Case([900, 70], None, kv=2, group=group, dim=dim, page=page)
+    if wide:
+        case.widen()
+    case.ks.fill_(1.0)
+    case.vs.fill_(1.0)
+    k = torch.zeros(case.k.shape, device="cuda")
+    k[..., 0] = case.randn(*case.k.shape[:3]).clamp(-1, 1)
+    q = torch.zeros(2, case.kv * group, dim, device="cuda")
+    q[..., 0] = size * (1 + torch.rand(2, case.kv * group, generator=case.gen, device="cuda"))
+    best = [333, 68]
+    for b, at in enumerate(best):
+        k[int(case.block_table[b, at // page]), :, at % page, 0] = 3.25
+    case.k.copy_(k.to(E4M3))
+    got = _attention(case, q.to(BF16), softmax_scale=0.7)
+    for b, at in enumerate(best):
+        value = case.v[int(case.block_table[b, at // page]), :, at % page].float()
+        assert torch.equal(got[b].float(), value.repeat_interleave(group, 0))

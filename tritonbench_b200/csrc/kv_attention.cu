@@ -115,6 +115,9 @@ __device__ __forceinline__ float exp2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// 2^(v f - ref), the product rounded as it was for the largest one that ref comes from: the largest p is 2^kBelow however
+// large the scores are (in a fused multiply-add the product's rounding error, 64 at 2^30, is left over in the argument)
+__device__ __forceinline__ float exp2_of(float v, float f, float ref) { return exp2_approx(__fsub_rn(__fmul_rn(v, f), ref)); }
 __device__ __forceinline__ bool has_nan_code(uint32_t w) {  // any byte 0x7f or 0xff
   const uint32_t m = (w & 0x7f7f7f7fu) + 0x01010101u;
   return (m & 0x80808080u) != 0;
@@ -714,16 +717,16 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
             in0 = fmaxf(in0, fmaxf(s[mt][nt][0], s[mt][nt][2]));
             in1 = fmaxf(in1, fmaxf(s[mt][nt][1], s[mt][nt][3]));
           }
-          top0 = S::kSubs == 1 ? in0 : fmaxf(top0, in0 * k_scale[sub]);
-          top1 = S::kSubs == 1 ? in1 : fmaxf(top1, in1 * k_scale[sub]);
+          top0 = S::kSubs == 1 ? in0 : fmaxf(top0, in0 * (col[nt].x * k_scale[sub]));
+          top1 = S::kSubs == 1 ? in1 : fmaxf(top1, in1 * (col[nt].y * k_scale[sub]));
         }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
           top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
           top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
         }
-        top[nt][0] = top0 * (S::kSubs == 1 ? col[nt].x * k_scale[0] : col[nt].x);
-        top[nt][1] = top1 * (S::kSubs == 1 ? col[nt].y * k_scale[0] : col[nt].y);
+        top[nt][0] = S::kSubs == 1 ? top0 * (col[nt].x * k_scale[0]) : top0;
+        top[nt][1] = S::kSubs == 1 ? top1 * (col[nt].y * k_scale[0]) : top1;
         passed = passed || top[nt][0] > m[nt][0] + (kBelow + kSlack) || top[nt][1] > m[nt][1] + (kBelow + kSlack);
       }
       if (__any_sync(0xffffffffu, passed)) {
@@ -783,8 +786,8 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
           const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
-          const float p0 = exp2_approx(fmaf(s[mt][nt][0], e0, -ref0)), p1 = exp2_approx(fmaf(s[mt][nt][1], e1, -ref1));
-          const float p2 = exp2_approx(fmaf(s[mt][nt][2], e0, -ref0)), p3 = exp2_approx(fmaf(s[mt][nt][3], e1, -ref1));
+          const float p0 = exp2_of(s[mt][nt][0], e0, ref0), p1 = exp2_of(s[mt][nt][1], e1, ref1);
+          const float p2 = exp2_of(s[mt][nt][2], e0, ref0), p3 = exp2_of(s[mt][nt][3], e1, ref1);
           // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Scores of 2^23 and more are
           // a unit off in fp32, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
           pf[mt][nt][0] = finite_half2_of(p0, p1);
