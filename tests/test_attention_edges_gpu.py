@@ -94,3 +94,30 @@ def test_scores_that_fp32_holds_in_steps_of_several_units(cuda_device, size, dim
     for b, at in enumerate(best):
         value = case.v[int(case.block_table[b, at // page]), :, at % page].float()
         assert torch.equal(got[b].float(), value.repeat_interleave(group, 0))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dim,page,group", [(64, 16, 1), (64, 32, 9), (128, 16, 8), (128, 64, 12), (256, 16, 4)])
+def test_log_sum_exp_is_that_of_unrounded_weights(cuda_device, dim, page, group, wide):
+    """The last token of every sequence well above the others, scores of one exact product each and below 16 in units of
+    log2.  The factor on them is off by 3 * 2^-24 of itself (the scale, log2 e, their product), the argument of exp2 by one more
+    rounding and exp2 by 2^-22.  A lane sums every 32nd token at most, and 16 sums join lanes, warps and blocks: 2^-24 each.
+    Then log2, its sum with the reference, ln 2 and the product: at most 2^-23 of a value below 32 each."""
+    lens = [260 + 37 * i for i in range(20)]
+    case = Case(lens, None, kv=2, group=group, dim=dim, page=page, dtype=BF16)
+    if wide:
+        case.widen()
+    case.ks.fill_(1.0)
+    score = torch.zeros(case.k.shape, device="cuda")
+    score[..., 0] = case.randn(*case.k.shape[:3])
+    for b, n in enumerate(lens):
+        score[int(case.block_table[b, (n - 1) // page]), :, (n - 1) % page, 0] = 4 + b / 8
+    case.k.copy_(score.to(E4M3))
+    q = torch.zeros(case.tokens, case.kv * group, dim, device="cuda")
+    q[..., 0] = (1 + 0.25 * torch.rand(q.shape[:2], generator=case.gen, device="cuda")) * dim**0.5
+    q = q.to(BF16)
+    _, want, _, _ = _plain_attention(case, q, dim**-0.5)
+    _, lse = _attention(case, q, return_lse=True)
+    bound = 4 * 2.0**-24 * 16 + 2.0**-22 + (max(lens) / 32 + 16) * 2.0**-24 + 4 * 32 * 2.0**-23
+    assert bound < 2.0**-15  # weights rounded to fp16 are off by up to 2^-11 each
+    assert (lse.double() - want).abs().max() <= bound, float((lse.double() - want).abs().max())

@@ -255,9 +255,9 @@ __device__ __forceinline__ int token_of(int i) {
   return i ^ ((i & 1) << 2);                                                  // 0 5 2 7, 4 1 6 3
 }
 
-// part of a tile in the workspace: O [kRows][kD], then (max, sum) [kRows][2]
+// part of a tile in the workspace: O [kRows][kD], then (reference, sum) [kRows][2], then the sum for the log-sum-exp [kRows]
 template <int kRows, int kD>
-__host__ __device__ constexpr size_t part_floats() { return static_cast<size_t>(kRows) * (kD + 2); }
+__host__ __device__ constexpr size_t part_floats() { return static_cast<size_t>(kRows) * (kD + 3); }
 
 // A tile that CTAs first_cta to last_cta share (first_cta -1: none).
 struct SharedTile {
@@ -283,16 +283,17 @@ __device__ __forceinline__ uint32_t pack_out2(float lo, float hi, bool fp16) {
   return r;
 }
 
-// Four elements of an output row from its sums, and the row's log-sum-exp (once, with the row's first elements).
+// Four elements of an output row from its sums, and the row's log-sum-exp from the sum of p before its rounding (once, with
+// the row's first elements).
 __device__ __forceinline__ void store_row(const KvAttentionParams& p, int q_base, int kv_head, int row, int d, float4 acc,
-                                          float top, float sum) {
+                                          float top, float sum, float exact) {
   const int token = row / p.group;
   const int head = kv_head * p.group + row - token * p.group;
   const float inv = sum == 0.0f ? 0.0f : __fdividef(1.0f, sum);  // no token seen: zeros
   uint16_t* at = static_cast<uint16_t*>(p.out) + (q_base + static_cast<long long>(token)) * p.o_token + head * p.o_head + d;
   *reinterpret_cast<uint2*>(at) = make_uint2(pack_out2(acc.x * inv, acc.y * inv, p.fp16), pack_out2(acc.z * inv, acc.w * inv, p.fp16));
   if (p.lse != nullptr && d == 0) {
-    p.lse[(q_base + static_cast<long long>(token)) * p.heads + head] = (top + log2f(sum)) * kLn2;
+    p.lse[(q_base + static_cast<long long>(token)) * p.heads + head] = (top + log2f(exact)) * kLn2;
   }
 }
 
@@ -322,6 +323,11 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {  // the sa
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+__device__ __forceinline__ float load_cluster1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -333,8 +339,11 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
   return v;
 }
 
-// kClustered: a cluster per tile (see run_t), else the shared list.
-template <int kD, int kNT, int kSub, bool kClustered>
+// kClustered: a cluster per tile (see run_t), else the shared list.  kLse: the log-sum-exp is asked for.  The output divides
+// by the sum of p as it was rounded to fp16 (what a row's largest p is off by then cancels); the log-sum-exp is that of p in
+// fp32, a second sum.  Device us without / with it: 64 requests 95.9 / 95.9, 48 requests with heads of 64 66.2 / 67.9, drafted
+// tokens (16 rows a tile, no register to spare) 94.0 / 100.2, so the other calls do without.
+template <int kD, int kNT, int kSub, bool kClustered, bool kLse>
 __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attention_kernel(const KvAttentionParams p) {
   using S = Shape<kD, kNT, kSub>;
   using C = Cursor<S::kRows, S::kUnit>;
@@ -487,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   char* const queries = smem + S::kRingBytes;
   float4* const own_rows = reinterpret_cast<float4*>(queries + S::kQBytes);  // clustered: what this CTA found, unnormalised
   __shared__ float2 own_ml[S::kRows];
+  __shared__ float join_exact[kWarps][kLse ? S::kRows : 1], own_exact[kLse ? S::kRows : 1];
 
   int next_page = -1;  // lane i: page of part i of the chunk that is requested next, loaded one step early
   const auto look_up = [&]() {
@@ -610,11 +620,11 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) o[h][i][nt][0] = o[h][i][nt][1] = o[h][i][nt][2] = o[h][i][nt][3] = 0.0f;
     float v_unit = 1.0f, v_top = 1.0f;  // unit of o, the largest so far
-    float m[kNT][2], l[kNT][2];
+    float m[kNT][2], l[kNT][2], exact[kNT][2];  // reference, sum of p as it was rounded, sum of p
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       m[nt][0] = m[nt][1] = kMinusInf;
-      l[nt][0] = l[nt][1] = 0.0f;
+      l[nt][0] = l[nt][1] = exact[nt][0] = exact[nt][1] = 0.0f;
     }
 
     for (int unit = unit0; unit < unit_end; ++unit) {
@@ -741,6 +751,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
               f[c] = exp2_approx(m[nt][c] - to);
               m[nt][c] = to;
               l[nt][c] *= f[c];
+              if constexpr (kLse) exact[nt][c] *= f[c];
             }
           }
 #pragma unroll
@@ -794,6 +805,10 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
           pf[mt][nt][1] = finite_half2_of(p2, p3);
           add_halves(l[nt][0], l[nt][1], pf[mt][nt][0]);
           add_halves(l[nt][0], l[nt][1], pf[mt][nt][1]);
+          if constexpr (kLse) {
+            exact[nt][0] += p0 + p2;
+            exact[nt][1] += p1 + p3;
+          }
         }
         if (S::kSubs > 1 && mixed) {
 #pragma unroll
@@ -933,10 +948,14 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+        for (int x = 4; x < 32; x <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+          if constexpr (kLse) exact[nt][c] += __shfl_xor_sync(0xffffffffu, exact[nt][c], x);
+        }
         if (g == 0) {
           join_ml[warp][8 * nt + 2 * t + c][0] = m[nt][c];
           join_ml[warp][8 * nt + 2 * t + c][1] = l[nt][c];
+          if constexpr (kLse) join_exact[warp][8 * nt + 2 * t + c] = exact[nt][c];
         }
       }
 #pragma unroll
@@ -966,12 +985,13 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_ml[w][r][0]);
         const float ref = top == kMinusInf ? 0.0f : top;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float sum = 0.0f;
+        float sum = 0.0f, all = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float f = exp2_approx(join_ml[w][r][0] - ref);
           const float4 v = join_row(w, in)[d ^ ((r >> 1) & 3)];
           sum = fmaf(join_ml[w][r][1], f, sum);
+          if constexpr (kLse) all = fmaf(join_exact[w][r], f, all);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
           acc.z = fmaf(v.z, f, acc.z);
@@ -979,14 +999,18 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
         if constexpr (kClustered) {
           own_rows[r * (kD / 4) + d] = acc;
-          if (d == 0) own_ml[r] = make_float2(top, sum);
+          if (d == 0) {
+            own_ml[r] = make_float2(top, sum);
+            if constexpr (kLse) own_exact[r] = all;
+          }
         } else if (begins && ends) {
-          store_row(p, cur.s.q_base, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum);
+          store_row(p, cur.s.q_base, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum, all);
         } else {
           reinterpret_cast<float4*>(part)[r * (kD / 4) + d] = acc;
           if (d == 0) {
             part[S::kRows * kD + 2 * r] = top;
             part[S::kRows * kD + 2 * r + 1] = sum;
+            if constexpr (kLse) part[S::kRows * (kD + 2) + r] = all;
           }
         }
       }
@@ -1008,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
     }
     cluster_sync();
     const int vecs = rows * (kD / 4), end = vecs * (rank + 1) / p.cluster;
-    const uint32_t rows_at = smem_addr(own_rows), ml_at = smem_addr(own_ml);
+    const uint32_t rows_at = smem_addr(own_rows), ml_at = smem_addr(own_ml), exact_at = smem_addr(own_exact);
     for (int i = vecs * rank / p.cluster + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
       const int r = i / (kD / 4), d = i % (kD / 4);
       float2 ml[kMaxCluster];
@@ -1020,20 +1044,21 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
       }
       const float ref = top == kMinusInf ? 0.0f : top;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float sum = 0.0f;
+      float sum = 0.0f, all = 0.0f;
 #pragma unroll
       for (int c = 0; c < kMaxCluster; ++c) {
         if (!(ml[c].y == 0.0f)) {  // a CTA that saw nothing may have left its rows unwritten (NaN: it saw something)
           const float f = exp2_approx(ml[c].x - ref);
           const float4 v = load_cluster4(in_cta(rows_at + 16 * i, c));
           sum = fmaf(ml[c].y, f, sum);
+          if constexpr (kLse) all = fmaf(load_cluster1(in_cta(exact_at + 4 * r, c)), f, all);
           acc.x = fmaf(v.x, f, acc.x);
           acc.y = fmaf(v.y, f, acc.y);
           acc.z = fmaf(v.z, f, acc.z);
           acc.w = fmaf(v.w, f, acc.w);
         }
       }
-      store_row(p, cur.s.q_base, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum);
+      store_row(p, cur.s.q_base, cur.kv_head, cur.row0 + r, 4 * d, acc, top, sum, all);
     }
     cluster_sync();  // nobody leaves while others read its memory
   }
@@ -1045,17 +1070,19 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
 constexpr int kGroups = 8, kAhead = 4;
 
 struct RunningSum {
-  float top, sum;
+  float top, sum, exact;
   float4 acc;
   __device__ __forceinline__ void move_to(float ref) {  // ref not below top
     const float f = exp2_approx(top - (ref == kMinusInf ? 0.0f : ref));
     top = ref;
     sum *= f;
+    exact *= f;
     acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
   }
-  __device__ __forceinline__ void add(float m, float l, float4 v) {  // m not above top
+  __device__ __forceinline__ void add(float m, float l, float all, float4 v) {  // m not above top
     const float f = exp2_approx(m - (top == kMinusInf ? 0.0f : top));
     sum = fmaf(l, f, sum);
+    exact = fmaf(all, f, exact);
     acc.x = fmaf(v.x, f, acc.x);
     acc.y = fmaf(v.y, f, acc.y);
     acc.z = fmaf(v.z, f, acc.z);
@@ -1068,6 +1095,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   constexpr int kRows = 8 * kNT, kVecs = kD / 4;
   __shared__ float4 group_acc[kJoinThreads];
   __shared__ float2 group_ml[kJoinThreads];
+  __shared__ float group_exact[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Split* splits = static_cast<const Split*>(p.workspace);
   const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + p.parts_offset);
@@ -1078,6 +1106,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   const int role = static_cast<int>(threadIdx.x) / kThreadsOfRole, thread = static_cast<int>(threadIdx.x) % kThreadsOfRole;
   float4* const role_acc = group_acc + role * kThreadsOfRole;
   float2* const role_ml = group_ml + role * kThreadsOfRole;
+  float* const role_exact = group_exact + role * kThreadsOfRole;
   const auto sync = [&]() {
     __syncwarp();
     asm volatile("bar.sync %0, %1;" ::"r"(1 + role), "n"(kThreadsOfRole) : "memory");
@@ -1096,18 +1125,21 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
       const int groups = min(min(kThreadsOfRole / n, kGroups), count);
       const int group = thread / n, vec = at + thread % n;
       const int r = vec / kVecs, d = vec % kVecs;
-      RunningSum run = {kMinusInf, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+      RunningSum run = {kMinusInf, 0.0f, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
       if (group < groups) {
         for (int c0 = group; c0 < count; c0 += groups * kAhead) {
           float2 ml[kAhead];
+          float all[kAhead];
           float4 v[kAhead];
 #pragma unroll
           for (int x = 0; x < kAhead; ++x) {
             const int c = c0 + x * groups;
             ml[x] = make_float2(kMinusInf, 0.0f);
             v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            all[x] = 0.0f;
             if (c < count) {
               ml[x] = *reinterpret_cast<const float2*>(part(c) + kRows * kD + 2 * r);
+              if (p.lse != nullptr) all[x] = part(c)[kRows * (kD + 2) + r];
               v[x] = reinterpret_cast<const float4*>(part(c))[vec];
             }
           }
@@ -1116,12 +1148,13 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
           for (int x = 0; x < kAhead; ++x) ref = fmaxf(ref, ml[x].x);
           run.move_to(ref);
 #pragma unroll
-          for (int x = 0; x < kAhead; ++x) run.add(ml[x].x, ml[x].y, v[x]);
+          for (int x = 0; x < kAhead; ++x) run.add(ml[x].x, ml[x].y, all[x], v[x]);
         }
       }
       if (groups > 1) {
         role_acc[thread] = run.acc;
         role_ml[thread] = make_float2(run.top, run.sum);
+        role_exact[thread] = run.exact;
         sync();
       }
       if (group == 0) {
@@ -1130,9 +1163,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
         run.move_to(ref);
         for (int x = 1; x < groups; ++x) {
           const float2 ml = role_ml[thread + x * n];
-          run.add(ml.x, ml.y, role_acc[thread + x * n]);
+          run.add(ml.x, ml.y, role_exact[thread + x * n], role_acc[thread + x * n]);
         }
-        store_row(p, sp.q_base, sp.kv_head, sp.row0 + r, 4 * d, run.acc, run.top, run.sum);
+        store_row(p, sp.q_base, sp.kv_head, sp.row0 + r, 4 * d, run.acc, run.top, run.sum, run.exact);
       }
       if (groups > 1) sync();
     }
@@ -1157,18 +1190,19 @@ cudaError_t make_plan(Plan* plan) {
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   int ctas = ctas_per_device[dev].load();
   if (ctas == 0) {
-    const auto kernel = kv_attention_kernel<kD, kNT, kSub, false>;
+    const auto kernel = kv_attention_kernel<kD, kNT, kSub, false, false>;
     int sms = 0, per_sm = 0;
     err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (err != cudaSuccess) return err;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
-    if (err != cudaSuccess) return err;
+    const auto allow = [](const void* f, int smem) { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); };
+    const auto address = [](auto f) { return reinterpret_cast<const void*>(f); };
+    if ((err = allow(address(kernel), S::kSmemBytes)) != cudaSuccess) return err;
+    if ((err = allow(address(kv_attention_kernel<kD, kNT, kSub, false, true>), S::kSmemBytes)) != cudaSuccess) return err;
+    if ((err = allow(address(kv_attention_kernel<kD, kNT, kSub, true, false>), S::kClusteredSmemBytes)) != cudaSuccess) return err;
+    if ((err = allow(address(kv_attention_kernel<kD, kNT, kSub, true, true>), S::kClusteredSmemBytes)) != cudaSuccess) return err;
     err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, S::kSmemBytes);
     if (err != cudaSuccess) return err;
     if (per_sm < 1) return cudaErrorInvalidConfiguration;
-    err = cudaFuncSetAttribute(kv_attention_kernel<kD, kNT, kSub, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               S::kClusteredSmemBytes);
-    if (err != cudaSuccess) return err;
     ctas = sms * per_sm;
     ctas_per_device[dev] = ctas;
   }
@@ -1212,11 +1246,15 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_attention_kernel<kD, kNT, kSub, true>, p);
+    return cudaLaunchKernelEx(&cfg, p.lse != nullptr ? kv_attention_kernel<kD, kNT, kSub, true, true> : kv_attention_kernel<kD, kNT, kSub, true, false>, p);
   }
   if (params.workspace_bytes < plan.bytes) return cudaErrorMemoryAllocation;
   p.parts_offset = plan.parts_offset;
-  kv_attention_kernel<kD, kNT, kSub, false><<<plan.ctas, kThreads, S::kSmemBytes, stream>>>(p);
+  if (p.lse != nullptr) {
+    kv_attention_kernel<kD, kNT, kSub, false, true><<<plan.ctas, kThreads, S::kSmemBytes, stream>>>(p);
+  } else {
+    kv_attention_kernel<kD, kNT, kSub, false, false><<<plan.ctas, kThreads, S::kSmemBytes, stream>>>(p);
+  }
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   // may be resident before the first kernel has ended; it waits for it (griddepcontrol.wait)

@@ -580,7 +580,8 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     (a decode step, drafted tokens, a chunk of a prompt).  q [tokens, heads, head_dim] bf16 or fp16; heads / kv_heads
     neighbouring query heads share a kv head; block_table, seq_lens, cu_seqlens as for fp8_kv_append, which has stored the
     tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
-    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads].  out may be q.
+    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads] (of weights in fp32; the
+    weights that multiply v are rounded to fp16).  out may be q.
 
     Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
     (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows behind
