@@ -121,3 +121,31 @@ def test_log_sum_exp_is_that_of_unrounded_weights(cuda_device, dim, page, group,
     bound = 4 * 2.0**-24 * 16 + 2.0**-22 + (max(lens) / 32 + 16) * 2.0**-24 + 4 * 32 * 2.0**-23
     assert bound < 2.0**-15  # weights rounded to fp16 are off by up to 2^-11 each
     assert (lse.double() - want).abs().max() <= bound, float((lse.double() - want).abs().max())
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dim,page,group", [(64, 16, 1), (64, 16, 9), (64, 32, 3), (128, 16, 8), (128, 16, 12), (256, 16, 2)])
+def test_value_scales_that_are_no_powers_of_two(cuda_device, dim, page, group, wide):
+    """Pages of one chunk whose V scales differ by factors that fp16 does not hold, and a token 30 above all others: the output
+    is its value.  The others weigh e^-30 each; p goes to fp16 once, with the page's share of the largest scale, and what that
+    rounding is off by cancels, so that a handful of fp32 roundings are left."""
+    case = Case([900, 70, 333, 64] * 4, None, kv=2, group=group, dim=dim, page=page, dtype=FP16)
+    if wide:
+        case.widen()
+    case.ks.fill_(1.0)
+    case.vs.copy_(1 + 6 * torch.rand(case.vs.shape, generator=case.gen, device="cuda"))
+    k = torch.zeros(case.k.shape, device="cuda")
+    want = torch.zeros(case.tokens, case.kv, dim, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(case.lens):
+        at = (37 * b + 5) % n
+        page_no, row = int(case.block_table[b, at // page]), at % page
+        k[page_no, :, row, 0] = 30.0
+        want[b] = case.v[page_no, :, row].double() * case.vs[page_no].double()[:, None]
+    case.k.copy_(k.to(E4M3))
+    q = torch.zeros(case.tokens, case.kv * group, dim, device="cuda", dtype=FP16)
+    q[..., 0] = 1.0
+    off = (_attention(case, q, softmax_scale=1.0).double() - want.repeat_interleave(group, 1)).abs()
+    want = want.abs().repeat_interleave(group, 1)
+    bound = 8 * 2.0**-23 * want + 900 * math.exp(-30) * 448 * 7
+    limit = bound + _half_step(FP16) * (want + bound) + TINY[FP16]
+    assert (off <= limit).all(), float((off - limit).max())

@@ -110,6 +110,11 @@ __device__ __forceinline__ void add_halves(float& lo, float& hi, uint32_t h) {
       : "+f"(lo), "+f"(hi)
       : "r"(h));
 }
+__device__ __forceinline__ void add_halves(float& lo, float& hi, uint32_t h, float times) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  lo = fmaf(v.x, times, lo);
+  hi = fmaf(v.y, times, hi);
+}
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -766,8 +771,9 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
       }
       // V scales: O is kept in units of the chunk's largest one, so that products can be added to it where they are; p is
-      // multiplied by what a page's scale is of that, down to an eighth: exact for scales that are powers of two (which are
-      // mostly alike), else two more roundings to fp16.
+      // multiplied by what a page's scale is of that, down to an eighth: in fp16 where the scales are powers of two (as the
+      // append makes them; exact down to subnormals), else in fp32 before the one rounding to fp16 (48 requests with heads of
+      // 64 and pages of 16, a call: 74 us when all chunks with different scales did that, 69.7 so, 68.7 with fp16 for all).
       float v_max = 0.0f;
 #pragma unroll
       for (int sub = 0; sub < S::kSubs; ++sub) v_max = there[sub] ? fmaxf(v_max, v_scale[sub]) : v_max;
@@ -781,40 +787,58 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
         }
       }
       mixed = mixed && plain;
-      uint32_t share[S::kSubs];  // of the largest scale, twice in fp16
+      float share[S::kSubs];  // of the largest scale
+      bool odd = false;       // some share is no power of two
       if (S::kSubs > 1 && mixed) {
         const float inv = 1.0f / v_max;
 #pragma unroll
         for (int sub = 0; sub < S::kSubs; ++sub) {
-          const float f = there[sub] ? v_scale[sub] * inv : 1.0f;
-          share[sub] = half2_of(f, f);
+          share[sub] = there[sub] ? v_scale[sub] * inv : 1.0f;
+          odd = odd || (__float_as_uint(share[sub]) & 0x7fffffu) != 0;
         }
       }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         // a column without a token so far: any finite reference will do
         const float ref0 = m[nt][0] == kMinusInf ? 0.0f : m[nt][0], ref1 = m[nt][1] == kMinusInf ? 0.0f : m[nt][1];
+        // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Scores of 2^23 and more are a
+        // unit off in fp32, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
+        const auto weights = [&](auto by_share) {
 #pragma unroll
-        for (int mt = 0; mt < S::kMT; ++mt) {
-          const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
-          const float p0 = exp2_of(s[mt][nt][0], e0, ref0), p1 = exp2_of(s[mt][nt][1], e1, ref1);
-          const float p2 = exp2_of(s[mt][nt][2], e0, ref0), p3 = exp2_of(s[mt][nt][3], e1, ref1);
-          // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Scores of 2^23 and more are
-          // a unit off in fp32, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
-          pf[mt][nt][0] = finite_half2_of(p0, p1);
-          pf[mt][nt][1] = finite_half2_of(p2, p3);
-          add_halves(l[nt][0], l[nt][1], pf[mt][nt][0]);
-          add_halves(l[nt][0], l[nt][1], pf[mt][nt][1]);
-          if constexpr (kLse) {
-            exact[nt][0] += p0 + p2;
-            exact[nt][1] += p1 + p3;
+          for (int mt = 0; mt < S::kMT; ++mt) {
+            const float e0 = col[nt].x * k_scale[mt * 16 / kSub], e1 = col[nt].y * k_scale[mt * 16 / kSub];
+            const float p0 = exp2_of(s[mt][nt][0], e0, ref0), p1 = exp2_of(s[mt][nt][1], e1, ref1);
+            const float p2 = exp2_of(s[mt][nt][2], e0, ref0), p3 = exp2_of(s[mt][nt][3], e1, ref1);
+            if constexpr (by_share.value) {
+              const float f = share[mt * 16 / kSub], back = 1.0f / f;
+              pf[mt][nt][0] = finite_half2_of(p0 * f, p1 * f);
+              pf[mt][nt][1] = finite_half2_of(p2 * f, p3 * f);
+              add_halves(l[nt][0], l[nt][1], pf[mt][nt][0], back);
+              add_halves(l[nt][0], l[nt][1], pf[mt][nt][1], back);
+            } else {
+              pf[mt][nt][0] = finite_half2_of(p0, p1);
+              pf[mt][nt][1] = finite_half2_of(p2, p3);
+              add_halves(l[nt][0], l[nt][1], pf[mt][nt][0]);
+              add_halves(l[nt][0], l[nt][1], pf[mt][nt][1]);
+            }
+            if constexpr (kLse) {
+              exact[nt][0] += p0 + p2;
+              exact[nt][1] += p1 + p3;
+            }
           }
-        }
-        if (S::kSubs > 1 && mixed) {
+        };
+        if (S::kSubs > 1 && odd) {
+          weights(std::true_type{});
+        } else {
+          weights(std::false_type{});
+          if (S::kSubs > 1 && mixed) {
 #pragma unroll
-          for (int mt = 0; mt < S::kMT; ++mt)
+            for (int mt = 0; mt < S::kMT; ++mt) {
+              const uint32_t f = half2_of(share[mt * 16 / kSub], share[mt * 16 / kSub]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(pf[mt][nt][i]) : "r"(share[mt * 16 / kSub]));
+              for (int i = 0; i < 2; ++i) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(pf[mt][nt][i]) : "r"(f));
+            }
+          }
         }
 #pragma unroll
         for (int mt = 0; mt < S::kMT; ++mt) {
