@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import BF16, E4M3, FP16, TINY, Case, _check_append, _check_attention, _context, _half_step, _plain_attention, _qkv
+from test_attention_gpu import BF16, E4M3, FP16, TINY, Case, _check_append, _check_attention, _context, _half_step, _plain_attention, _qkv, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,16 @@ def test_value_scales_that_are_no_powers_of_two(cuda_device, dim, page, group, w
     bound = 8 * 2.0**-23 * want + 900 * math.exp(-30) * 448 * 7
     limit = bound + _half_step(FP16) * (want + bound) + TINY[FP16]
     assert (off <= limit).all(), float((off - limit).max())
+
+
+@pytest.mark.parametrize("lens", [[-1], [5, -1, 0, -2, -(2**31), 70]])
+def test_rows_of_negative_lengths_are_zero(cuda_device, lens):
+    """A padded entry may have any length below one; its row of a given q_out is zeroed, also where q_out is q."""
+    from tritonbench_b200 import ops
+
+    case = Case(lens, None, kv=2, group=2, dim=64, page=32)
+    q, k, v = _qkv(case)
+    for q_out in (torch.full_like(q, 3.0), q):
+        got = _check_append(case, q, k, v, _table(128, 64), q_out=q_out)
+        assert got is q_out
+    assert not ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens)[[n <= 0 for n in lens]].any()

@@ -292,7 +292,7 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
     const long long t = token0 + i;
     long long pos;
     if (p.cu_seqlens == nullptr) {
-      pos = p.seq_lens[t] - 1ll;
+      pos = max(p.seq_lens[t] - 1ll, -1ll);
     } else if (t >= p.cu_seqlens[p.batch]) {
       pos = -2;  // behind the last sequence
     } else {
