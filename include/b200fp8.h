@@ -289,8 +289,8 @@ typedef struct b200fp8_kv_batch {
  * a page and head is the smallest power of two (>= 2^-126) that takes the largest finite magnitude of its tokens to at
  * most 448; when a page that already holds tokens needs a larger one, their codes are multiplied by old / new scale.
  * Infinities and NaN are stored as NaN.  dtype of q, k, v: bf16 or fp16; element pitches per token and head, multiples
- * of 8.  q_out rows of skipped tokens are zero; rows behind the last sequence are left as they were, or zeroed with
- * fill_rest.  Two sequences must not append to the same page.
+ * of 8.  q_out rows of skipped tokens are zero; rows that no sequence has (in front of cu_seqlens[0], behind
+ * cu_seqlens[batch]) are left as they were, or zeroed with fill_rest.  Two sequences must not append to the same page.
  */
 int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t heads, int64_t q_token,
                       int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t qo_token,
@@ -302,7 +302,7 @@ int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, 
  * heads share a kv head,  o = sum_j softmax_j(softmax_scale * q . k_j) v_j.  q and out [tokens, heads, head_dim] bf16 or
  * fp16, element pitches multiples of 8 (out: of 4); lse [tokens, heads] fp32 (natural logarithm of the softmax's
  * denominator) or NULL.  A row without a token to see gives zeros, and lse = -infinity.  fill_rest as above for out; lse is
- * -infinity behind the last sequence.
+ * -infinity in rows that no sequence has.
  * (tokens * heads / kv_heads / 8 + batch) * kv_heads * (table_width * page_size / 64 + 3) must be below 2^31.
  * The workspace needs no initialisation and may be reused as soon as the call has run; calls that overlap need one each.
  * Small calls need none: b200fp8_kv_attention_workspace_bytes is 0 then (also where the call itself would return an

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import BF16, E4M3, FP16, TINY, Case, _check_append, _check_attention, _context, _half_step, _plain_attention, _qkv, _table
+from test_attention_gpu import (BF16, E4M3, FP16, TINY, Case, _bytes, _check_append, _check_attention, _context, _half_step,
+                                _plain_attention, _qkv, _table)
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +163,41 @@ def test_rows_of_negative_lengths_are_zero(cuda_device, lens):
         got = _check_append(case, q, k, v, _table(128, 64), q_out=q_out)
         assert got is q_out
     assert not ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens)[[n <= 0 for n in lens]].any()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("first,batch", [(1, 3), (37, 3), (40, 1)])
+def test_rows_in_front_of_the_first_sequence(cuda_device, first, batch, wide):
+    """Bounds that do not begin at zero, a slice of a larger batch's: the rows in front belong to no sequence, like those
+    behind the last one."""
+    from tritonbench_b200 import ops
+
+    lens, new = [90, 40, 33][:batch], [5, 40, 2][:batch]
+    case = Case(lens, new, kv=2, group=3, dim=64, page=16)
+    table = _table(128, 64)
+    q, k, v = _qkv(case, extra=2)
+    front = [torch.cat([case.randn(first, *t.shape[1:]).to(t.dtype), t]) for t in (q, k, v)]
+    start = case.snapshot()
+    want_q = _check_append(case, q, k, v, table)
+    want = case.snapshot()
+    for t, old in zip((case.k, case.v, case.ks, case.vs), start):
+        t.view(torch.uint8).copy_(old.view(torch.uint8)) if t.dtype is E4M3 else t.copy_(old)
+    cu = case.cu + first
+    got = ops.fp8_kv_append(*front, case.cache, case.block_table, case.seq_lens, cu, table)
+    for t, w in zip((case.k, case.v, case.ks, case.vs), want):
+        assert torch.equal(_bytes(t), _bytes(w)) if t.dtype is E4M3 else torch.equal(t, w)
+    assert torch.equal(got[first:], want_q) and not got[:first].any()
+    given = torch.full_like(front[0], 3.0)
+    ops.fp8_kv_append(*front, case.cache, case.block_table, case.seq_lens, cu, table, q_out=given)
+    assert (given[:first] == 3.0).all() and (given[-2:] == 3.0).all() and torch.equal(given[first:-2], want_q[:-2])
+    if wide:
+        case.widen()
+    args = (case.cache, case.block_table, case.seq_lens)
+    want, want_lse = ops.fp8_kv_attention(want_q, *args, case.cu, return_lse=True)
+    torch.full_like(got, 5.0)  # what a fresh result may find in its memory
+    out, lse = ops.fp8_kv_attention(got, *args, cu, return_lse=True)
+    assert torch.equal(out[first:], want) and torch.equal(lse[first:], want_lse)
+    assert not out[:first].any() and (lse[:first] == -math.inf).all()
+    out, lse = ops.fp8_kv_attention(got, *args, cu, out=given.fill_(3.0), return_lse=True)
+    assert out is given and (out[:first] == 3.0).all() and (out[-2:] == 3.0).all() and torch.equal(out[first:-2], want[:-2])
+    assert (lse[:first] == -math.inf).all() and torch.equal(lse[first:], want_lse)

@@ -324,7 +324,7 @@ struct KvAppendParams {
   int batch, tokens, heads, kv_heads, dim, rot;
   int page_size, page_shift, table_width, num_pages;
   int dtype, interleaved;
-  int fill_rest;  // rows of q_out behind the last sequence are zeroed (else left as they are)
+  int fill_rest;  // rows of q_out that no sequence has are zeroed (else left as they are)
 };
 cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream);
 

@@ -293,8 +293,8 @@ __device__ __forceinline__ void rotate_q(const KvAppendParams& p, long long bloc
     long long pos;
     if (p.cu_seqlens == nullptr) {
       pos = max(p.seq_lens[t] - 1ll, -1ll);
-    } else if (t >= p.cu_seqlens[p.batch]) {
-      pos = -2;  // behind the last sequence
+    } else if (t < p.cu_seqlens[0] || t >= p.cu_seqlens[p.batch]) {
+      pos = -2;  // no sequence's
     } else {
       const int b = search_sequence(p.batch, t, [&](int s) { return static_cast<long long>(p.cu_seqlens[s]); });
       pos = p.seq_lens[b] - static_cast<long long>(p.cu_seqlens[b + 1]) + t;

@@ -302,14 +302,14 @@ __device__ __forceinline__ void store_row(const KvAttentionParams& p, int q_base
   }
 }
 
-// Rows behind the last sequence: zeros (where asked for), and nothing to see.
+// Rows in front of the first sequence and behind the last one: zeros (where asked for), and nothing to see.
 template <int kD>
-__device__ __forceinline__ void fill_behind(const KvAttentionParams& p, int threads) {
+__device__ __forceinline__ void fill_rest(const KvAttentionParams& p, int threads) {
   if (p.cu_seqlens == nullptr || (!p.fill_rest && p.lse == nullptr)) return;
-  const int used = min(max(p.cu_seqlens[p.batch], 0), p.tokens);
-  const long long n = static_cast<long long>(p.tokens - used) * p.heads;
+  const int first = min(max(p.cu_seqlens[0], 0), p.tokens), end = min(max(p.cu_seqlens[p.batch], first), p.tokens);
+  const long long n = static_cast<long long>(first + p.tokens - end) * p.heads;
   for (long long r = blockIdx.x; r < n; r += gridDim.x) {
-    const long long token = used + r / p.heads;
+    const long long at = r / p.heads, token = at < first ? at : at - first + end;
     const int head = static_cast<int>(r % p.heads);
     uint16_t* o = static_cast<uint16_t*>(p.out) + token * p.o_token + head * p.o_head;
     if (p.fill_rest) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
   Shares shares(0, 1);
   int run_end = 0;
   if constexpr (kClustered) {
-    fill_behind<kD>(p, kThreads);
+    fill_rest<kD>(p, kThreads);
     const int slot = cta / p.cluster;  // (row tile, kv head)
     const int row_slot = slot / p.kv_heads, kv_head = slot - row_slot * p.kv_heads;
     int row_tile;
@@ -1124,7 +1124,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   const Split* splits = static_cast<const Split*>(p.workspace);
   const float* parts = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + p.parts_offset);
   const int cta = static_cast<int>(blockIdx.x);
-  fill_behind<kD>(p, kJoinThreads);
+  fill_rest<kD>(p, kJoinThreads);
   // half of the threads take the tile that this CTA continued, half the one that it began
   constexpr int kThreadsOfRole = kJoinThreads / 2;
   const int role = static_cast<int>(threadIdx.x) / kThreadsOfRole, thread = static_cast<int>(threadIdx.x) % kThreadsOfRole;

@@ -516,7 +516,7 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     448.  A page that already holds tokens keeps its scale, or is moved to a larger one.  Infinities and NaN are stored as
     NaN.  Rows whose position would be negative (seq_lens[b] = 0: a padded entry), positions behind the block table and
     pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q) keeps its rows
-    behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to twice in one call (two sequences
+    in front of cu_seqlens[0] and behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to twice in one call (two sequences
     that share one, or a sequence that has it twice)."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
@@ -584,8 +584,8 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     weights that multiply v are rounded to fp16).  out may be q.
 
     Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
-    (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows behind
-    cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for up to a few dozen new
+    (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows in front
+    of cu_seqlens[0] and behind cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for up to a few dozen new
     tokens a sequence: the cache is read once per 16 query rows, with the work split over the context.  The result does
     not depend on timing.  Small calls need no workspace, the others allocate theirs, so captured graphs and streams never
     share one."""
