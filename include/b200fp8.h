@@ -272,7 +272,8 @@ typedef struct b200fp8_kv_cache {
  * host): the rows of q, k, v are the newest tokens of `batch` sequences packed behind one another, those of sequence b
  * from cu_seqlens[b] to cu_seqlens[b + 1] - one each when cu_seqlens is NULL.  seq_lens[b] is the length of the sequence
  * with them, so its last row is at position seq_lens[b] - 1.  Position j lies in row j % page_size of page
- * block_table[b * table_pitch + j / page_size].  Rows whose position would be negative (seq_lens[b] smaller than the
+ * block_table[b * table_pitch + j / page_size] (table_pitch: any that is not negative, 0 when all sequences have the same
+ * pages).  Rows whose position would be negative (seq_lens[b] smaller than the
  * number of rows; 0 for a padded entry of the batch), positions beyond the table's width and pages outside the cache
  * are skipped: nothing is stored for them or read there.
  */

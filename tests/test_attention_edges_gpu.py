@@ -201,3 +201,23 @@ def test_rows_in_front_of_the_first_sequence(cuda_device, first, batch, wide):
     out, lse = ops.fp8_kv_attention(got, *args, cu, out=given.fill_(3.0), return_lse=True)
     assert out is given and (out[:first] == 3.0).all() and (out[-2:] == 3.0).all() and torch.equal(out[first:-2], want[:-2])
     assert (lse[:first] == -math.inf).all() and torch.equal(lse[first:], want_lse)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_sequences_that_share_a_row_of_the_block_table(cuda_device, wide):
+    """Attention of several sequences over the same pages, by a table whose rows are one, or overlap."""
+    from tritonbench_b200 import ops
+
+    case = Case([300], None, kv=2, group=3, dim=64, page=16)
+    if wide:
+        case.widen()
+    lens = torch.tensor([300, 17, 0, 128, 299], dtype=torch.int32, device="cuda")
+    q = case.randn(5, 6, 64).bfloat16()
+    table = case.block_table.expand(5, -1)
+    assert table.stride(0) == 0
+    want = ops.fp8_kv_attention(q, case.cache, table.contiguous(), lens)
+    assert torch.equal(ops.fp8_kv_attention(q, case.cache, table, lens), want)
+    windows = case.block_table[0].as_strided((5, table.shape[1] - 8), (2, 1))  # sequence b begins with page 2 b
+    lens = lens.clamp(max=16 * 8)
+    want = ops.fp8_kv_attention(q, case.cache, windows.contiguous(), lens)
+    assert torch.equal(ops.fp8_kv_attention(q, case.cache, windows, lens), want)

@@ -929,10 +929,10 @@ int check_kv(const b200fp8_kv_cache* c, const b200fp8_kv_batch* r, int64_t heads
   if (r->cu_seqlens == nullptr && r->tokens != r->batch) return B200FP8_BAD_ARG;
   if (r->tokens == 0) return B200FP8_OK;
   if (r->batch == 0 || r->seq_lens == nullptr) return B200FP8_BAD_ARG;
-  if (r->table_width > 0 && (r->block_table == nullptr || (r->batch > 1 && r->table_pitch < r->table_width))) return B200FP8_BAD_ARG;
+  if (r->table_width > 0 && (r->block_table == nullptr || (r->batch > 1 && r->table_pitch < 0))) return B200FP8_BAD_ARG;
   if (c->num_pages > 0 && (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr)) return B200FP8_BAD_ARG;
   if (heads > 0xFFFFll || c->num_pages > 0x7FFFFFFFll || r->batch > 0xFFFFFFll || r->tokens > 0x3FFFFFFFll ||
-      r->tokens * heads > 0x3FFFFFFFll || r->table_width * c->page_size > 0x3FFFFFFFll) {
+      r->tokens * heads > 0x3FFFFFFFll || r->table_width > 0x3FFFFFFFll || r->table_width * c->page_size > 0x3FFFFFFFll) {
     return B200FP8_TOO_LARGE;
   }
   if (!aligned16(c->k) || !aligned16(c->v)) return B200FP8_UNSUPPORTED_ALIGNMENT;

@@ -496,7 +496,7 @@ def _pack_batch(tokens: int, cache: Fp8KvCache, block_table: torch.Tensor, seq_l
         if cu_seqlens.get_device() != device:
             raise ValueError("cu_seqlens must be on the cache's device")
         cu = cu_seqlens.data_ptr()
-    return _lib.KV_BATCH.pack(block_table.data_ptr(), seq_lens.data_ptr(), cu, pitch if pitch > width else width, width, batch, tokens)
+    return _lib.KV_BATCH.pack(block_table.data_ptr(), seq_lens.data_ptr(), cu, pitch, width, batch, tokens)
 
 
 def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tensor,
@@ -578,8 +578,8 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
     """Attention of the newest tokens of every sequence over the cache, each token over itself and all before it
     (a decode step, drafted tokens, a chunk of a prompt).  q [tokens, heads, head_dim] bf16 or fp16; heads / kv_heads
-    neighbouring query heads share a kv head; block_table, seq_lens, cu_seqlens as for fp8_kv_append, which has stored the
-    tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
+    neighbouring query heads share a kv head; block_table (any stride between its rows: sequences over the same pages may share one),
+    seq_lens, cu_seqlens as for fp8_kv_append, which has stored the tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
     return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads] (of weights in fp32; the
     weights that multiply v are rounded to fp16).  out may be q.
 
