@@ -291,7 +291,8 @@ typedef struct b200fp8_kv_batch {
  * most 448; when a page that already holds tokens needs a larger one, their codes are multiplied by old / new scale.
  * Infinities and NaN are stored as NaN.  dtype of q, k, v: bf16 or fp16; element pitches per token and head, multiples
  * of 8.  q_out rows of skipped tokens are zero; rows that no sequence has (in front of cu_seqlens[0], behind
- * cu_seqlens[batch]) are left as they were, or zeroed with fill_rest.  Two sequences must not append to the same page.
+ * cu_seqlens[batch]) are left as they were, or zeroed with fill_rest.  Two sequences must not append to the same page, and no two pages, heads or rows of the cache
+ * may lie in the same place (pitches of zero are refused; attention takes them).
  */
 int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t heads, int64_t q_token,
                       int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t qo_token,

@@ -40,3 +40,28 @@ def test_table_pitches_that_the_library_takes(cdll, ptr):
     assert call(-1) == lib.BAD_ARG
     assert call(0) == call(1) == call(2) == lib.UNSUPPORTED_ALIGNMENT
     assert call(1 << 40, width=1 << 60) == lib.TOO_LARGE
+
+
+def test_append_refuses_pitches_of_zero(cdll, ptr):
+    """One scale, or one row of codes, of several pages or heads would be read and written by several blocks at once."""
+    def call(pitches, scale_pitches, pages=4, heads=2):
+        cache = lib.KV_CACHE.pack(ptr, ptr, ptr, ptr, *pitches, *pitches, *scale_pitches, *scale_pitches, pages, heads, 16, 64)
+        rows = lib.KV_BATCH.pack(ptr, ptr, 0, 2, 2, 1, 1)
+        # q on an odd address: refused, but after the cache
+        return cdll.b200fp8_kv_append(ptr + 2, ptr, ptr, ptr, 0, 4, 256, 64, 128, 64, 128, 64, 256, 64, cache, rows, None, 0, 0, 0, 0, None)
+
+    good, scales = (2048, 1024, 64), (2, 1)
+    assert call(good, scales) == lib.UNSUPPORTED_ALIGNMENT
+    for i in range(3):
+        assert call([0 if i == j else p for j, p in enumerate(good)], scales) == lib.BAD_ARG
+    assert call(good, (0, 1)) == call(good, (2, 0)) == lib.BAD_ARG
+    assert call((0, 0, 64), (0, 0), pages=1, heads=1) == lib.UNSUPPORTED_ALIGNMENT  # pitches that are never used
+
+
+def test_tensors_whose_elements_are_one():
+    x = torch.zeros(4, 3, 16, 64)
+    for t in (x, x.transpose(1, 2), x[:, 1:2], x[::2, :, :, ::4], x[..., :48], x.unflatten(0, (2, 2))[:, 1], torch.zeros(1).expand(1, 1)):
+        assert not ops._elements_share_memory(t)
+    for t in (x[:1].expand(4, 3, 16, 64), x[:, :1].expand(4, 3, 16, 64), torch.zeros(4, 1).expand(4, 3), torch.zeros(1).expand(2),
+              torch.zeros(200).as_strided((3, 64), (32, 1))):
+        assert ops._elements_share_memory(t)

@@ -221,3 +221,29 @@ def test_sequences_that_share_a_row_of_the_block_table(cuda_device, wide):
     lens = lens.clamp(max=16 * 8)
     want = ops.fp8_kv_attention(q, case.cache, windows.contiguous(), lens)
     assert torch.equal(ops.fp8_kv_attention(q, case.cache, windows, lens), want)
+
+
+def test_caches_that_share_memory_are_read_but_not_appended_to(cuda_device):
+    from tritonbench_b200 import ops
+
+    case = Case([60, 33], None, kv=2, group=2, dim=64, page=16)
+    q, k, v = _qkv(case)
+    q, one = q.contiguous(), case.k[:, :1].expand(case.k.shape)
+    scale = case.ks[:, :1].expand(case.ks.shape)
+    caches = [(one, case.v, case.ks, case.vs), (case.k, case.v, scale, case.vs), (case.k, case.v, case.ks, case.vs[:1].expand(case.vs.shape)),
+              (case.k, case.k, case.ks, case.vs), (case.k, case.v, case.ks, case.ks)]
+    before = case.snapshot()
+    for tensors in caches:
+        cache = ops.Fp8KvCache(*tensors)
+        with pytest.raises(ValueError, match="appended"):
+            ops.fp8_kv_append(q, k, v, cache, case.block_table, case.seq_lens)
+        own = ops.Fp8KvCache(*(t.contiguous().clone() for t in tensors))
+        assert torch.equal(ops.fp8_kv_attention(q, cache, case.block_table, case.seq_lens),
+                           ops.fp8_kv_attention(q, own, case.block_table, case.seq_lens))
+    for t, old in zip((case.k, case.v, case.ks, case.vs), before):
+        assert torch.equal(_bytes(t), _bytes(old)) if t.dtype is E4M3 else torch.equal(t, old)
+    both = torch.zeros(7, 2, 2, 16, 64, dtype=torch.uint8, device="cuda").view(E4M3)  # k and v beside each other in one tensor
+    cache = ops.Fp8KvCache(both[:, 0], both[:, 1], *(torch.zeros(7, 2, 2, device="cuda").unbind(1)))
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[:6].view(2, 3)
+    ops.fp8_kv_append(q, k, v, cache, table, torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
+    assert not cache.read_only and both.view(torch.uint8).any()

@@ -1003,6 +1003,12 @@ int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, 
   if (k == nullptr || v == nullptr || (q != nullptr && q_out == nullptr)) return B200FP8_BAD_ARG;
   if (table != nullptr && (rot % 16 != 0 || !aligned16(table))) return B200FP8_UNSUPPORTED_ALIGNMENT;
   const int64_t kv = cache->kv_heads, tokens = rows->tokens;
+  const int64_t counts[3] = {cache->num_pages, kv, cache->page_size};
+  for (int i = 0; i < 3; ++i) {  // what is written must not be one for several pages, heads or rows
+    if (counts[i] < 2) continue;
+    if (cache->k_pitch[i] == 0 || cache->v_pitch[i] == 0) return B200FP8_BAD_ARG;
+    if (i < 2 && (cache->k_scale_pitch[i] == 0 || cache->v_scale_pitch[i] == 0)) return B200FP8_BAD_ARG;
+  }
   if (!aligned16(k) || !aligned16(v) || uneven(tokens, k_token | v_token, 8) || uneven(kv, k_head | v_head, 8)) {
     return B200FP8_UNSUPPORTED_ALIGNMENT;
   }

@@ -427,13 +427,25 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     return out
 
 
+def _elements_share_memory(t: torch.Tensor) -> bool:
+    """Whether some elements of t are one (an expanded or overlapping view); also true of a few layouts that interleave
+    their dimensions, which no cache has."""
+    extent = 0  # offset of the last element of the dimensions so far
+    for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= extent:
+            return True
+        extent += stride * (n - 1)
+    return False
+
+
 class Fp8KvCache:
     """A paged key/value cache in e4m3: k and v [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn (any page, head
     and row strides that are multiples of 16 and below 2^31; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads]
     float32; a value is code * scale, no scale is negative.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object
-    describes the four tensors and keeps them alive; make one with `empty`, or around tensors of your own."""
+    describes the four tensors and keeps them alive; make one with `empty`, or around tensors of your own.  Tensors that are
+    expanded, overlap or are one (k and v) can be read, but not appended to."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor", "read_only")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         for t, name in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
@@ -458,6 +470,8 @@ class Fp8KvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
         self.device = k.get_device()
+        self.read_only = pages > 0 and (any(_elements_share_memory(t) for t in (k, v, k_scale, v_scale))
+                                        or k.data_ptr() == v.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr())
         self.descriptor = _lib.KV_CACHE.pack(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3],
             *k_scale.stride(), *v_scale.stride(), pages, heads, size, dim)
@@ -520,6 +534,8 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     that share one, or a sequence that has it twice)."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
+    if cache.read_only:
+        raise ValueError("the cache's tensors are expanded, overlap or are one: such a cache can be read, but not appended to")
     device, heads, dim = cache.device, cache.kv_heads, cache.head_dim
     dtype = k.dtype
     if k.get_device() != device or v.get_device() != device:
