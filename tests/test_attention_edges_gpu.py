@@ -247,3 +247,21 @@ def test_caches_that_share_memory_are_read_but_not_appended_to(cuda_device):
     table = torch.arange(7, dtype=torch.int32, device="cuda")[:6].view(2, 3)
     ops.fp8_kv_append(q, k, v, cache, table, torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
     assert not cache.read_only and both.view(torch.uint8).any()
+
+
+def test_the_tensors_of_a_cache_cannot_be_replaced(cuda_device):
+    """The kernels use the addresses that the cache was made with: another tensor in its place would not be seen."""
+    from tritonbench_b200 import ops
+
+    cache = ops.Fp8KvCache.empty(4, 2, 64, 16)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        old = getattr(cache, name)
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, old.clone())
+        with pytest.raises(AttributeError, match=name):
+            delattr(cache, name)
+        assert getattr(cache, name) is old
+    for name in ("num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor", "read_only", "other"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, 1)
+    assert (cache.num_pages, cache.kv_heads, cache.page_size, cache.head_dim, cache.device) == (4, 2, 16, 64, 0)

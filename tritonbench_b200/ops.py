@@ -442,8 +442,9 @@ class Fp8KvCache:
     """A paged key/value cache in e4m3: k and v [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn (any page, head
     and row strides that are multiples of 16 and below 2^31; head_dim contiguous), k_scale and v_scale [num_pages, kv_heads]
     float32; a value is code * scale, no scale is negative.  page_size 16, 32, 64 or 128; head_dim 64, 128 or 256.  The object
-    describes the four tensors and keeps them alive; make one with `empty`, or around tensors of your own.  Tensors that are
-    expanded, overlap or are one (k and v) can be read, but not appended to."""
+    describes the four tensors and keeps them alive; make one with `empty`, or around tensors of your own.  Its attributes
+    cannot be replaced, and the tensors' memory must not be (`set_`, `.data`, `resize_`): make another cache instead.  Tensors that
+    are expanded, overlap or are one (k and v) can be read, but not appended to."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "kv_heads", "page_size", "head_dim", "device", "descriptor", "read_only")
 
@@ -467,14 +468,20 @@ class Fp8KvCache:
         for t in (k, v):
             if t.data_ptr() % 16 or any(st % 16 for st, n in zip(t.stride()[:3], t.shape) if n > 1):
                 raise NotImplementedError("rows of k and v must start on 16-byte boundaries")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
-        self.device = k.get_device()
-        self.read_only = pages > 0 and (any(_elements_share_memory(t) for t in (k, v, k_scale, v_scale))
-                                        or k.data_ptr() == v.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr())
-        self.descriptor = _lib.KV_CACHE.pack(
+        read_only = pages > 0 and (any(_elements_share_memory(t) for t in (k, v, k_scale, v_scale))
+                                   or k.data_ptr() == v.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr())
+        descriptor = _lib.KV_CACHE.pack(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3],
             *k_scale.stride(), *v_scale.stride(), pages, heads, size, dim)
+        for name, value in zip(self.__slots__, (k, v, k_scale, v_scale, pages, heads, size, dim, k.get_device(), descriptor, read_only)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        # the descriptor holds addresses: with another tensor in its place the kernels would go on using the old one's memory
+        raise AttributeError(f"an Fp8KvCache's {name} cannot be replaced: make another cache")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"an Fp8KvCache's {name} cannot be removed")
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "Fp8KvCache":
