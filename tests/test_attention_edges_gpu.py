@@ -265,3 +265,27 @@ def test_the_tensors_of_a_cache_cannot_be_replaced(cuda_device):
         with pytest.raises(AttributeError):
             setattr(cache, name, 1)
     assert (cache.num_pages, cache.kv_heads, cache.page_size, cache.head_dim, cache.device) == (4, 2, 16, 64, 0)
+
+
+def test_copies_of_a_cache_describe_their_own_tensors(cuda_device):
+    import copy
+    import pickle
+
+    from tritonbench_b200 import ops
+
+    case = Case([60, 33], None, kv=2, group=2, dim=64, page=16)
+    q, k, v = _qkv(case)
+    before = case.snapshot()
+    want = ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens)
+    shallow, deep, loaded = copy.copy(case.cache), copy.deepcopy(case.cache), pickle.loads(pickle.dumps(case.cache))
+    assert shallow.k is case.k and shallow.descriptor == case.cache.descriptor
+    for c in (deep, loaded):
+        assert c.k.data_ptr() != case.k.data_ptr()
+        ops.fp8_kv_append(q, k * 2, v, c, case.block_table, case.seq_lens)
+        assert not torch.equal(_bytes(c.k), _bytes(before[0]))
+        assert torch.equal(_bytes(case.k), _bytes(before[0])) and torch.equal(case.vs, before[3])
+    case.v.view(torch.uint8).zero_()
+    assert not ops.fp8_kv_attention(q, case.cache, case.block_table, case.seq_lens).any()
+    deep = copy.deepcopy(shallow)
+    deep.v.view(torch.uint8).copy_(before[1].view(torch.uint8))
+    assert torch.equal(ops.fp8_kv_attention(q, deep, case.block_table, case.seq_lens), want)

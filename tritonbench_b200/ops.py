@@ -483,6 +483,12 @@ class Fp8KvCache:
     def __delattr__(self, name):
         raise AttributeError(f"an Fp8KvCache's {name} cannot be removed")
 
+    def __copy__(self):
+        return self
+
+    def __reduce__(self):  # a deep or pickled copy describes its own tensors (codes as bytes: torch cannot load 8-bit floats)
+        return _cache_of_bytes, (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale)
+
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "Fp8KvCache":
         """A cache without tokens (codes and scales zero)."""
@@ -490,6 +496,10 @@ class Fp8KvCache:
         k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
         ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
         return cls(k, v, ks, vs)
+
+
+def _cache_of_bytes(k, v, k_scale, v_scale) -> Fp8KvCache:
+    return Fp8KvCache(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), k_scale, v_scale)
 
 
 def _pack_batch(tokens: int, cache: Fp8KvCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
