@@ -4,8 +4,8 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import (BF16, E4M3, FP16, TINY, Case, _bytes, _check_append, _check_attention, _context, _half_step,
-                                _plain_attention, _qkv, _table)
+from test_attention_gpu import (BF16, E4M3, FP16, FP32, TINY, Case, _bytes, _check_append, _check_attention, _check_rotated, _context,
+                                _half_step, _plain_attention, _qkv, _table)
 
 pytestmark = pytest.mark.gpu
 
@@ -289,3 +289,59 @@ def test_copies_of_a_cache_describe_their_own_tensors(cuda_device):
     deep = copy.deepcopy(shallow)
     deep.v.view(torch.uint8).copy_(before[1].view(torch.uint8))
     assert torch.equal(ops.fp8_kv_attention(q, deep, case.block_table, case.seq_lens), want)
+
+
+def test_calls_without_a_gradient_refuse_to_drop_one(cuda_device):
+    from tritonbench_b200 import ops
+
+    case = Case([40, 64], None, kv=2, group=2, dim=64, page=64)
+    q, k, v = (t.clone() for t in _qkv(case))
+    table, args = _table(64, 64), (case.cache, case.block_table, case.seq_lens)
+    want_q = ops.fp8_kv_append(q, k, v, *args)
+    want = ops.fp8_kv_attention(q, *args)
+    for i in range(3):
+        given = [t.clone().requires_grad_() if j == i else t for j, t in enumerate((q, k, v))]
+        with pytest.raises(ValueError, match="gradient"):
+            ops.fp8_kv_append(*given, *args)
+        with torch.no_grad():
+            assert torch.equal(ops.fp8_kv_append(*given, *args), want_q)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.fp8_kv_append(q, k, v, *args, table=table.clone().requires_grad_())
+    leaf = q.clone().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        ops.fp8_kv_attention(leaf, *args)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.fp8_kv_attention(leaf * 2, *args)
+    with torch.no_grad():
+        assert torch.equal(ops.fp8_kv_attention(leaf, *args), want)
+    with torch.inference_mode():
+        assert torch.equal(ops.fp8_kv_attention(leaf, *args), want)
+    x, pos = torch.randn(2, 3, 64, device="cuda"), torch.arange(2, device="cuda")
+    with pytest.raises(ValueError, match="gradient"):
+        ops.rotary(x, pos, table.clone().requires_grad_())
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: ops.fp8_kv_attention(dual, *args), lambda: ops.fp8_kv_append(dual, k, v, *args)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        assert torch.equal(ops.fp8_kv_attention(q, *args), want)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_rotary_carries_forward_tangents(cuda_device, dtype, interleaved):
+    from tritonbench_b200 import ops
+
+    fwd = torch.autograd.forward_ad
+    x, step = (torch.randn(7, 3, 64, device="cuda").to(dtype) for _ in range(2))
+    pos, table = torch.randint(0, 64, (7,), device="cuda"), _table(64, 32)
+    for transpose in (False, True):
+        with fwd.dual_level():
+            y = ops.rotary(fwd.make_dual(x, step), pos, table, interleaved, transpose)
+            value, tangent = fwd.unpack_dual(y)
+            assert tangent is not None
+            _check_rotated(value, x, pos, table, interleaved, transpose)
+            _check_rotated(tangent, step, pos, table, interleaved, transpose)
+            with pytest.raises(ValueError, match="differentiable"):
+                ops.rotary(fwd.make_dual(x, step), pos, table, out=torch.empty_like(x))
+            assert fwd.unpack_dual(ops.rotary(x, pos, table)).tangent is None

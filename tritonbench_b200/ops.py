@@ -9,6 +9,7 @@ a fresh bf16 [M, N] tensor as the result.
 from typing import Callable, Dict, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import lib as _lib
 
@@ -357,10 +358,22 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must not be expanded: several of its elements are one")
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _refuse_gradients(what: str, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor) -> None:
+    """The cache holds codes, so these calls have no gradient; a result that looks like a constant must not pass for one."""
+    recorded = (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)) and torch.is_grad_enabled()
+    if recorded or (_forward_ad._current_level >= 0 and _has_tangent(q, k, v)):
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, table, interleaved, transpose):
         ctx.save_for_backward(positions, table)
+        ctx.save_for_forward(positions, table)
         ctx.form = (interleaved, transpose)
         return rotary(x, positions, table, interleaved, transpose)
 
@@ -372,6 +385,14 @@ class _Rotary(torch.autograd.Function):
             grad = grad.contiguous()
         return rotary(grad, positions, table, interleaved, not transpose), None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, x_tangent, *_):
+        positions, table = ctx.saved_tensors
+        interleaved, transpose = ctx.form
+        if x_tangent.stride(2) != 1:
+            x_tangent = x_tangent.contiguous()
+        return rotary(x_tangent, positions, table, interleaved, transpose)
+
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interleaved: bool = False,
            transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -380,7 +401,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     (2i, 2i + 1) if interleaved - of the first rot elements of a head, the others copied.  positions [tokens] int32 or
     int64; table float32 [max_positions, rot] from `rotary.rotary_table`; a position outside it gives NaN.
     fp32 arithmetic, one rounding.  out may be x.  transpose=True is the gradient with regard to x; a call on an x that
-    requires one is differentiable."""
+    requires one, or carries a forward tangent, is differentiable (with regard to x alone)."""
     device = x.get_device()
     if device < 0:
         _require_cuda(x, "x")
@@ -405,7 +426,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     max_pos, rot = table.shape
     if max_pos < 1 or not 2 <= rot <= dim or rot % 2:
         raise ValueError("the table needs a row, and an even width of at most dim")
-    if x.requires_grad and torch.is_grad_enabled():
+    tangents = _forward_ad._current_level >= 0
+    if (table.requires_grad and torch.is_grad_enabled()) or (tangents and _has_tangent(table)):
+        raise ValueError("rotary has no gradient with regard to its table: pass table.detach()")
+    if (x.requires_grad and torch.is_grad_enabled()) or (tangents and _has_tangent(x)):
         if out is not None:
             raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
         return _Rotary.apply(x, positions, table, interleaved, transpose)
@@ -547,8 +571,9 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     448.  A page that already holds tokens keeps its scale, or is moved to a larger one.  Infinities and NaN are stored as
     NaN.  Rows whose position would be negative (seq_lens[b] = 0: a padded entry), positions behind the block table and
     pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q) keeps its rows
-    in front of cu_seqlens[0] and behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to twice in one call (two sequences
-    that share one, or a sequence that has it twice)."""
+    in front of cu_seqlens[0] and behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to
+    twice in one call (two sequences that share one, or a sequence that has it twice).  There is no gradient: q, k or v that
+    require one are refused where gradients are recorded."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
     if cache.read_only:
@@ -561,6 +586,7 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
         raise ValueError(f"k and v must be [tokens, {heads}, {dim}]")
     if dtype is not torch.bfloat16 and dtype is not torch.float16 or v.dtype is not dtype:
         raise ValueError("k and v must be bfloat16 or float16, both the same")
+    _refuse_gradients("fp8_kv_append", q, k, v)
     tokens = k.shape[0]
     k_token, k_head, k_one = k.stride()
     v_token, v_head, v_one = v.stride()
@@ -592,6 +618,8 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
         max_pos, rot = table.shape
         if max_pos < 1 or not 2 <= rot <= dim or rot % 2:
             raise ValueError("the table needs a row, and an even width of at most head_dim")
+        if table.requires_grad and torch.is_grad_enabled():
+            raise ValueError("fp8_kv_append has no gradient with regard to its table: pass table.detach()")
         table_ptr = table.data_ptr()
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
     args = (q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, _DTYPES[dtype], heads, q_token, q_head, k_token, k_head, v_token, v_head,
@@ -611,17 +639,19 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
     """Attention of the newest tokens of every sequence over the cache, each token over itself and all before it
     (a decode step, drafted tokens, a chunk of a prompt).  q [tokens, heads, head_dim] bf16 or fp16; heads / kv_heads
-    neighbouring query heads share a kv head; block_table (any stride between its rows: sequences over the same pages may share one),
-    seq_lens, cu_seqlens as for fp8_kv_append, which has stored the tokens' own k and v before.  softmax_scale: head_dim ** -0.5 by default.  Returns out in q's dtype (fp32 inside), with
-    return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads] (of weights in fp32; the
-    weights that multiply v are rounded to fp16).  out may be q.
+    neighbouring query heads share a kv head; block_table (any stride between its rows: sequences over the same pages may
+    share one), seq_lens, cu_seqlens as for fp8_kv_append, which has stored the tokens' own k and v before.  softmax_scale:
+    head_dim ** -0.5 by default.  Returns out in q's dtype (sums in fp32; the weights that multiply v are rounded to fp16),
+    with return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads], of weights in fp32.
+    out may be q.
 
     Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
     (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows in front
-    of cu_seqlens[0] and behind cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for up to a few dozen new
-    tokens a sequence: the cache is read once per 16 query rows, with the work split over the context.  The result does
-    not depend on timing.  Small calls need no workspace, the others allocate theirs, so captured graphs and streams never
-    share one."""
+    of cu_seqlens[0] and behind cu_seqlens[-1] keep what they hold in a given `out`; in a fresh one they are zero.  Built for
+    up to a few dozen new tokens a sequence: the cache is read once per 16 query rows, with the work split over the context
+    (a prompt of thousands of tokens works, at that rate).  The result does not depend on timing.  Small calls need no
+    workspace, the others allocate theirs, so captured graphs and streams never share one.  There is no gradient: a q that
+    requires one is refused where gradients are recorded."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
     device = cache.device
@@ -632,6 +662,7 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
         raise ValueError(f"q must be [tokens, heads, {cache.head_dim}]")
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError("q must be bfloat16 or float16")
+    _refuse_gradients("fp8_kv_attention", None, q, q)
     tokens, heads, dim = q.shape
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads cannot share {cache.kv_heads} kv heads")
