@@ -345,3 +345,30 @@ def test_rotary_carries_forward_tangents(cuda_device, dtype, interleaved):
             with pytest.raises(ValueError, match="differentiable"):
                 ops.rotary(fwd.make_dual(x, step), pos, table, out=torch.empty_like(x))
             assert fwd.unpack_dual(ops.rotary(x, pos, table)).tangent is None
+
+
+def test_results_written_in_place_are_seen_by_autograd(cuda_device):
+    """A tensor that a backward pass still needs, and that a call has overwritten, must not give a wrong gradient."""
+    from tritonbench_b200 import ops
+
+    case = Case([40, 64], None, kv=2, group=2, dim=64, page=64)
+    q, k, v = (t.clone() for t in _qkv(case))
+    pos, table, args = torch.arange(2, device="cuda"), _table(64, 64), (case.cache, case.block_table, case.seq_lens)
+    calls = [lambda x: ops.rotary(x, pos, table, out=x), lambda x: ops.rotary(q, pos, table, out=x),
+             lambda x: ops.fp8_kv_append(x, k, v, *args, q_out=x), lambda x: ops.fp8_kv_attention(x, *args, out=x)]
+    for call in calls:
+        x = torch.randn_like(q)
+        w = torch.ones_like(q, requires_grad=True)
+        y = (w * x).sum()  # keeps x
+        call(x)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    leaf = torch.zeros_like(q).requires_grad_()
+    for call in (lambda: ops.rotary(q, pos, table, out=leaf), lambda: ops.fp8_kv_append(q, k, v, *args, q_out=leaf),
+                 lambda: ops.fp8_kv_attention(q, *args, out=leaf)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    assert not leaf.any()
+    with torch.inference_mode():
+        x = torch.randn_like(q)
+        assert ops.rotary(x, pos, table, out=x) is x

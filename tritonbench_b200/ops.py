@@ -351,11 +351,16 @@ def _fresh_like(x: torch.Tensor) -> torch.Tensor:
     return out if out.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _check_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+def _claim_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    """Checks a result that the caller gives, and tells autograd that it is written to: a backward pass that still needs what
+    it held must not go on without it."""
     if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device() or out.stride(2) != 1:
         raise ValueError(f"{name} must have the input's shape, dtype and device, the last dimension contiguous")
     if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{name} must not be expanded: several of its elements are one")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which these calls do not record for it")
+    torch.autograd.graph.increment_version(out)
 
 
 def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
@@ -436,7 +441,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     if out is None:
         out = _fresh_like(x)
     else:
-        _check_out(out, x, "out")
+        _claim_out(out, x, "out")
     if tokens == 0 or heads == 0:
         return out
     if device != torch.cuda.current_device():  # a launch on a stream of another device is an error
@@ -606,7 +611,7 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
         if q_out is None:
             q_out, fill = _fresh_like(q), 1
         else:
-            _check_out(q_out, q, "q_out")
+            _claim_out(q_out, q, "q_out")
         o_token, o_head, _ = q_out.stride()
         q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -673,7 +678,7 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     if out is None:
         out, fill = _fresh_like(q), 1
     else:
-        _check_out(out, q, "out")
+        _claim_out(out, q, "out")
     o_token, o_head, _ = out.stride()
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     rows = _pack_batch(tokens, cache, block_table, seq_lens, cu_seqlens)
