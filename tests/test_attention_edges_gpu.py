@@ -372,3 +372,12 @@ def test_results_written_in_place_are_seen_by_autograd(cuda_device):
     with torch.inference_mode():
         x = torch.randn_like(q)
         assert ops.rotary(x, pos, table, out=x) is x
+
+
+@pytest.mark.parametrize("batch", [4, 5, 6, 9, 12, 27])
+@pytest.mark.parametrize("dim,group", [(128, 16), (256, 8)])
+def test_calls_at_the_edge_of_what_is_resident(cuda_device, batch, dim, group):
+    """Batches for which the number of clusters that fit at once decides about their size, or against them; the clusters'
+    kernel has fewer blocks an SM than the other one here."""
+    case = Case([1024 - 100 * (b % 3) for b in range(batch)], None, kv=8, group=group, dim=dim, page=64)
+    _check_attention(case, case.randn(batch, 8 * group, dim).to(BF16))

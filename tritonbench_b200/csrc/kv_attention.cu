@@ -1196,23 +1196,45 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const K
   }
 }
 
+constexpr int kSmallUnits = 4;
+constexpr int kClusterSizes = 4;  // 1, 2, 4, 8
+
+// What the current device holds at once, per device (the same whoever asks first): CTAs of the list's kernel, and of the
+// other one in clusters of 1 << i.
+struct Residency {
+  std::atomic<int> ctas{0}, clustered[kClusterSizes] = {};
+};
 struct Plan {
   int ctas;
+  int clustered[kClusterSizes];
   size_t parts_offset, bytes;
 };
 
-// CTAs of a grid that fills the current device once, per device (the same whoever asks first)
-constexpr int kSmallUnits = 4;
+cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* attr, long long ctas, int cluster, int smem, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  *attr = {};
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
 
 template <int kD, int kNT, int kSub>
 cudaError_t make_plan(Plan* plan) {
   using S = Shape<kD, kNT, kSub>;
-  static std::atomic<int> ctas_per_device[64] = {};
+  static Residency per_device[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  int ctas = ctas_per_device[dev].load();
+  Residency& known = per_device[dev];
+  int ctas = known.ctas.load();
   if (ctas == 0) {
     const auto kernel = kv_attention_kernel<kD, kNT, kSub, false, false>;
     int sms = 0, per_sm = 0;
@@ -1227,10 +1249,19 @@ cudaError_t make_plan(Plan* plan) {
     err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, S::kSmemBytes);
     if (err != cudaSuccess) return err;
     if (per_sm < 1) return cudaErrorInvalidConfiguration;
+    for (int i = 0; i < kClusterSizes; ++i) {
+      int clusters = 0;
+      cudaLaunchAttribute attr;
+      const cudaLaunchConfig_t cfg = cluster_config(&attr, 1 << i, 1 << i, S::kClusteredSmemBytes, nullptr);
+      err = cudaOccupancyMaxActiveClusters(&clusters, kv_attention_kernel<kD, kNT, kSub, true, false>, &cfg);
+      if (err != cudaSuccess) return err;
+      known.clustered[i] = clusters << i;
+    }
     ctas = sms * per_sm;
-    ctas_per_device[dev] = ctas;
+    known.ctas = ctas;
   }
   plan->ctas = ctas;
+  for (int i = 0; i < kClusterSizes; ++i) plan->clustered[i] = known.clustered[i].load();
   plan->parts_offset = (static_cast<size_t>(ctas) * sizeof(Split) + 255) / 256 * 256;
   plan->bytes = plan->parts_offset + 2 * static_cast<size_t>(ctas) * part_floats<S::kRows, kD>() * sizeof(float);
   return cudaSuccess;
@@ -1247,29 +1278,24 @@ cudaError_t run_t(const KvAttentionParams& params, size_t* bytes, cudaStream_t s
   // CTA at most kSmallUnits units, up to 8 CTAs a tile.  It saves the second launch, the workspace and the list, about 2 us
   // on the device and 5 on the host, but shares nothing between tiles.  Device us, list / clusters: 1 sequence of 1024
   // tokens, 8 kv heads 8.0 / 5.9, of 4096 9.3 / 10.0 (4 units a CTA; the host takes 15.9 / 10.6), of 8192 11.1 / 14.8;
-  // 16 of 1024 13.6 / 12.4, of 2048 18.4 / 17.8 (ragged 14.3 / 17.5); 64 of 256, two waves, 14.7 / 17.8.
+  // 16 of 1024 13.6 / 12.4, of 2048 18.4 / 17.8 (ragged 14.3 / 17.5); 64 of 256, two waves, 14.7 / 17.8.  What is resident
+  // is asked of the clusters' own kernel, which needs more shared memory: 16 rows of 128 or 8 of 256 leave room for two of its
+  // blocks an SM where the list's has three.  5 sequences of 1024 tokens, 8 kv heads with 16 query heads each: clusters of 4,
+  // 10.8 us; clusters of 8 in two waves, by the list's figure, 16.6.
   const long long row_slots = p.cu_seqlens == nullptr ? static_cast<long long>(p.batch) * ((p.group + S::kRows - 1) / S::kRows)
                                                       : static_cast<long long>(p.tokens) * p.group / S::kRows + p.batch;
   const long long tiles = row_slots * p.kv_heads, units = p.max_len > S::kUnit ? (p.max_len + S::kUnit - 1) / S::kUnit : 1;
-  p.cluster = kMaxCluster;
-  while (p.cluster > 1 && (tiles * p.cluster > plan.ctas || p.cluster / 2 >= units)) p.cluster /= 2;
-  const bool clustered = tiles * p.cluster <= plan.ctas && units <= kSmallUnits * p.cluster;
+  int size = kClusterSizes - 1;
+  while (size > 0 && (tiles << size > plan.clustered[size] || (1 << size) / 2 >= units)) --size;
+  p.cluster = 1 << size;
+  const bool clustered = tiles << size <= plan.clustered[size] && units <= kSmallUnits * p.cluster;
   if (bytes != nullptr) {  // only asked for the size
     *bytes = clustered ? 0 : plan.bytes;
     return cudaSuccess;
   }
   if (clustered) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.cluster));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = S::kClusteredSmemBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(p.cluster);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(&attr, tiles * p.cluster, p.cluster, S::kClusteredSmemBytes, stream);
     return cudaLaunchKernelEx(&cfg, p.lse != nullptr ? kv_attention_kernel<kD, kNT, kSub, true, true> : kv_attention_kernel<kD, kNT, kSub, true, false>, p);
   }
   if (params.workspace_bytes < plan.bytes) return cudaErrorMemoryAllocation;
