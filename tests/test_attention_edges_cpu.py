@@ -7,6 +7,7 @@ import torch
 
 from test_attention_cpu import _cache
 from tritonbench_b200 import lib, ops
+from tritonbench_b200.rotary import rotary_frequencies
 
 
 @pytest.fixture(scope="module")
@@ -65,3 +66,10 @@ def test_tensors_whose_elements_are_one():
     for t in (x[:1].expand(4, 3, 16, 64), x[:, :1].expand(4, 3, 16, 64), torch.zeros(4, 1).expand(4, 3), torch.zeros(1).expand(2),
               torch.zeros(200).as_strided((3, 64), (32, 1))):
         assert ops._elements_share_memory(t)
+
+
+@pytest.mark.parametrize("base", [1.0, 0.5])
+def test_yarn_refuses_bases_whose_pairs_do_not_slow_down(base):
+    with pytest.raises(ValueError, match="base"):
+        rotary_frequencies(8, base=base, scaling="yarn", factor=4.0)
+    assert rotary_frequencies(8, base=base, scaling="linear", factor=4.0)[0].isfinite().all()

@@ -37,6 +37,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[st
         raise ValueError("original_max must be positive")
     turns = original_max * freq / (2 * math.pi)
     if scaling == "yarn":
+        if not base > 1:
+            raise ValueError("yarn scaling needs base > 1")
+
         def pair_with(n):  # the (fractional) pair that turns n times within original_max
             return rot_dim * math.log(original_max / (n * 2 * math.pi)) / (2 * math.log(base))
 
