@@ -1,5 +1,6 @@
 """Edges of the cache calls that are settled on the host: no GPU needed."""
 import ctypes
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -73,3 +74,17 @@ def test_yarn_refuses_bases_whose_pairs_do_not_slow_down(base):
     with pytest.raises(ValueError, match="base"):
         rotary_frequencies(8, base=base, scaling="yarn", factor=4.0)
     assert rotary_frequencies(8, base=base, scaling="linear", factor=4.0)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("original_max", [1, 5, 6, 7, 100, 300, 10**12])
+@pytest.mark.parametrize("rot", [2, 8, 128])
+def test_yarn_stretches_what_turns_less_than_once(rot, original_max):
+    plain, _ = rotary_frequencies(rot)
+    freq, _ = rotary_frequencies(rot, scaling="yarn", factor=4.0, original_max=original_max)
+    turns = original_max * plain / (2 * math.pi)
+    # the ramp begins and ends on whole pairs: one pair beyond either limit may lie on it
+    slow, fast = turns < 10000.0 ** (-2 / rot), turns > 32 * 10000.0 ** (2 / rot)
+    if original_max < 6:
+        slow = turns < 1
+    assert torch.equal(freq[slow], plain[slow] / 4) and torch.equal(freq[fast], plain[fast])
+    assert ((freq <= plain) & (freq >= plain / 4)).all()

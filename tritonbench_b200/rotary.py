@@ -44,7 +44,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[st
             return rot_dim * math.log(original_max / (n * 2 * math.pi)) / (2 * math.log(base))
 
         first, last = max(math.floor(pair_with(32.0)), 0), min(math.ceil(pair_with(1.0)), rot_dim - 1)
-        ramp = ((index / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
+        if last <= 0:  # no pair turns even once: all of them are stretched
+            ramp = torch.ones_like(freq)
+        else:
+            ramp = ((index / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
         return freq * (1 - ramp) + freq / factor * ramp, 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
     if scaling == "banded":
         if not high > low:
