@@ -381,3 +381,21 @@ def test_calls_at_the_edge_of_what_is_resident(cuda_device, batch, dim, group):
     kernel has fewer blocks an SM than the other one here."""
     case = Case([1024 - 100 * (b % 3) for b in range(batch)], None, kv=8, group=group, dim=dim, page=64)
     _check_attention(case, case.randn(batch, 8 * group, dim).to(BF16))
+
+
+def test_results_in_place_of_the_input_in_another_layout_are_refused(cuda_device):
+    """Same memory, tokens and heads exchanged: blocks would overwrite what others have not read yet."""
+    from tritonbench_b200 import ops
+
+    case = Case([40, 64, 5, 9], None, kv=2, group=2, dim=64, page=64)
+    q, k, v = (t.clone() for t in _qkv(case))
+    other, before, args = q.transpose(0, 1), q.clone(), (case.cache, case.block_table, case.seq_lens)
+    assert other.shape == q.shape and other.data_ptr() == q.data_ptr()
+    pos, table = torch.arange(4, device="cuda"), _table(64, 64)
+    for call in (lambda: ops.rotary(q, pos, table, out=other), lambda: ops.fp8_kv_append(q, k, v, *args, q_out=other),
+                 lambda: ops.fp8_kv_attention(q, *args, out=other)):
+        with pytest.raises(ValueError, match="layout"):
+            call()
+    assert torch.equal(q, before)
+    one = q[:1]  # a stride that leads nowhere may differ
+    assert ops.rotary(one, pos[:1], table, out=q.as_strided((1, 4, 64), (7, 64, 1))).data_ptr() == q.data_ptr()

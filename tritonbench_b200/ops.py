@@ -358,6 +358,9 @@ def _claim_out(out: torch.Tensor, like: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must have the input's shape, dtype and device, the last dimension contiguous")
     if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{name} must not be expanded: several of its elements are one")
+    if out is not like and out.data_ptr() == like.data_ptr() and any(
+            a != b for a, b, n in zip(out.stride(), like.stride(), out.shape) if n > 1) and out.numel():
+        raise ValueError(f"{name} must not lie where the input lies in another layout: elements would be overwritten unread")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which these calls do not record for it")
     torch.autograd.graph.increment_version(out)
@@ -405,7 +408,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     projection's output will do): y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for the pairs (i, i + rot/2) - or
     (2i, 2i + 1) if interleaved - of the first rot elements of a head, the others copied.  positions [tokens] int32 or
     int64; table float32 [max_positions, rot] from `rotary.rotary_table`; a position outside it gives NaN.
-    fp32 arithmetic, one rounding.  out may be x.  transpose=True is the gradient with regard to x; a call on an x that
+    fp32 arithmetic, one rounding.  out may be x, and must not overlap it otherwise.  transpose=True is the gradient with regard to x; a call on an x that
     requires one, or carries a forward tangent, is differentiable (with regard to x alone)."""
     device = x.get_device()
     if device < 0:
@@ -575,9 +578,10 @@ def fp8_kv_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, c
     One scale per page and kv head: the smallest power of two that takes the page's largest finite magnitude to at most
     448.  A page that already holds tokens keeps its scale, or is moved to a larger one.  Infinities and NaN are stored as
     NaN.  Rows whose position would be negative (seq_lens[b] = 0: a padded entry), positions behind the block table and
-    pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q) keeps its rows
-    in front of cu_seqlens[0] and behind cu_seqlens[-1]; in a fresh result they are zero.  A page must not be appended to
-    twice in one call (two sequences that share one, or a sequence that has it twice).  There is no gradient: q, k or v that
+    pages outside the cache are skipped, their q is zero where the position is negative.  q_out (may be q, and must not
+    overlap q, k and v otherwise) keeps its rows in front of cu_seqlens[0] and behind cu_seqlens[-1]; in a fresh result they
+    are zero.  A page must not be appended to twice in one call (two sequences that share one, or a sequence that has it
+    twice).  There is no gradient: q, k or v that
     require one are refused where gradients are recorded."""
     if not isinstance(cache, Fp8KvCache):
         raise ValueError("cache must be an Fp8KvCache")
@@ -648,7 +652,7 @@ def fp8_kv_attention(q: torch.Tensor, cache: Fp8KvCache, block_table: torch.Tens
     share one), seq_lens, cu_seqlens as for fp8_kv_append, which has stored the tokens' own k and v before.  softmax_scale:
     head_dim ** -0.5 by default.  Returns out in q's dtype (sums in fp32; the weights that multiply v are rounded to fp16),
     with return_lse also the natural logarithm of each softmax's denominator, float32 [tokens, heads], of weights in fp32.
-    out may be q.
+    out may be q, and must not overlap it otherwise.
 
     Rows that see no token (position negative, or seq_lens[b] = 0) are zero with lse -inf.  Pages outside the cache
     (-1 for a page that has been dropped) and positions behind the block table count as not there.  Rows in front
