@@ -400,7 +400,8 @@ cudaError_t launch_i(const KvAppendParams& p, cudaStream_t stream) {
   if (p.cu_seqlens == nullptr) return launch_t<T, kInterleaved, kWarps, 1, 1>(p, stream);
   // More pages than a wave of blocks (148 SMs x 4) and few tokens a sequence, or a prompt among many single tokens.  Device
   // us, this / a block a page / a warp a page: 64 sequences x 1 token 4.4 / 9.5 / 4.1, x 12 10.2 / 13.1 / 10.0, x 16 12.7 /
-  // 15.1, x 24 26.1 / 17.5 / 17.1; 63 x 1 and one of 400 9.3 / 12.9 / 22.6; 250 x 1 and one of 1500 24.5 / 38.7 / 33.6.
+  // 15.1, x 24 26.1 / 17.5 / 17.1; 63 x 1 and one of 400 9.3 / 12.9 / 22.6; 250 x 1 and one of 1500 24.5 / 38.7 / 33.6.  The
+  // rule goes by the average: 63 x 1 and one of 2048 takes a block a page, 23.5.
   // Fewer pages: 16 x 12 6.6 / 5.4, 8 x 6 5.1 / 4.5 / 4.9.
   if (works_of(p) > 592 && p.tokens <= 16ll * p.batch) return launch_t<T, kInterleaved, kEither, 1, 1>(p, stream);
   // Two slots a thread: a warp for 16 tokens of 64 (5000 tokens in such pages 16.5 us, a block each 31.2), a block for 64
