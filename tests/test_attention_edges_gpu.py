@@ -399,3 +399,20 @@ def test_results_in_place_of_the_input_in_another_layout_are_refused(cuda_device
     assert torch.equal(q, before)
     one = q[:1]  # a stride that leads nowhere may differ
     assert ops.rotary(one, pos[:1], table, out=q.as_strided((1, 4, 64), (7, 64, 1))).data_ptr() == q.data_ptr()
+
+
+def test_a_cache_with_attributes_of_its_own(cuda_device):
+    """A subclass may keep what it likes beside the tensors."""
+    from tritonbench_b200 import ops
+
+    class Named(ops.Fp8KvCache):
+        __slots__ = ("name", "free")
+
+    empty = ops.Fp8KvCache.empty(4, 2, 64, 16)
+    cache = Named(empty.k, empty.v, empty.k_scale, empty.v_scale)
+    cache.name, cache.free = "layer 3", [0, 1, 2, 3]
+    assert (cache.name, len(cache.free), cache.num_pages, cache.descriptor) == ("layer 3", 4, 4, empty.descriptor)
+    del cache.free
+    with pytest.raises(AttributeError, match="k_scale"):
+        cache.k_scale = empty.v_scale
+    assert isinstance(Named.empty(2, 1, 64, 16), Named)

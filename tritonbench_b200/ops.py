@@ -505,15 +505,19 @@ class Fp8KvCache:
         descriptor = _lib.KV_CACHE.pack(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3],
             *k_scale.stride(), *v_scale.stride(), pages, heads, size, dim)
-        for name, value in zip(self.__slots__, (k, v, k_scale, v_scale, pages, heads, size, dim, k.get_device(), descriptor, read_only)):
+        for name, value in zip(Fp8KvCache.__slots__, (k, v, k_scale, v_scale, pages, heads, size, dim, k.get_device(), descriptor, read_only)):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
         # the descriptor holds addresses: with another tensor in its place the kernels would go on using the old one's memory
-        raise AttributeError(f"an Fp8KvCache's {name} cannot be replaced: make another cache")
+        if name in Fp8KvCache.__slots__:
+            raise AttributeError(f"an Fp8KvCache's {name} cannot be replaced: make another cache")
+        object.__setattr__(self, name, value)
 
     def __delattr__(self, name):
-        raise AttributeError(f"an Fp8KvCache's {name} cannot be removed")
+        if name in Fp8KvCache.__slots__:
+            raise AttributeError(f"an Fp8KvCache's {name} cannot be removed")
+        object.__delattr__(self, name)
 
     def __copy__(self):
         return self
