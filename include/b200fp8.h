@@ -273,9 +273,9 @@ typedef struct b200fp8_kv_cache {
  * from cu_seqlens[b] to cu_seqlens[b + 1] - one each when cu_seqlens is NULL.  seq_lens[b] is the length of the sequence
  * with them, so its last row is at position seq_lens[b] - 1.  Position j lies in row j % page_size of page
  * block_table[b * table_pitch + j / page_size] (table_pitch: any that is not negative, 0 when all sequences have the same
- * pages).  Rows whose position would be negative (seq_lens[b] smaller than the
- * number of rows; 0 for a padded entry of the batch), positions beyond the table's width and pages outside the cache
- * are skipped: nothing is stored for them or read there.
+ * pages).  Rows whose position would be negative (seq_lens[b] smaller than the number of rows; 0 for a padded entry of the
+ * batch), positions beyond the table's width and pages outside the cache are skipped: nothing is stored for them or read
+ * there.  Rows in front of cu_seqlens[0] and behind cu_seqlens[batch] belong to no sequence.
  */
 typedef struct b200fp8_kv_batch {
   const int32_t* block_table;
@@ -290,9 +290,9 @@ typedef struct b200fp8_kv_batch {
  * a page and head is the smallest power of two (>= 2^-126) that takes the largest finite magnitude of its tokens to at
  * most 448; when a page that already holds tokens needs a larger one, their codes are multiplied by old / new scale.
  * Infinities and NaN are stored as NaN.  dtype of q, k, v: bf16 or fp16; element pitches per token and head, multiples
- * of 8.  q_out rows of skipped tokens are zero; rows that no sequence has (in front of cu_seqlens[0], behind
- * cu_seqlens[batch]) are left as they were, or zeroed with fill_rest.  Two sequences must not append to the same page, and no two pages, heads or rows of the cache
- * may lie in the same place (pitches of zero are refused; attention takes them).
+ * of 8.  q_out rows of negative positions are zero; rows that no sequence has are left as they were, or zeroed with
+ * fill_rest.  Two sequences must not append to the same page, and no two pages, heads or rows of the cache may lie in the
+ * same place (pitches of zero are refused; attention takes them).
  */
 int b200fp8_kv_append(const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t heads, int64_t q_token,
                       int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, int64_t qo_token,

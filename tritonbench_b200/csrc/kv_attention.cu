@@ -120,8 +120,9 @@ __device__ __forceinline__ float exp2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// 2^(v f - ref), the product rounded as it was for the largest one that ref comes from: the largest p is 2^kBelow however
-// large the scores are (in a fused multiply-add the product's rounding error, 64 at 2^30, is left over in the argument)
+// 2^(v f - ref), the product rounded as it was for the largest one that ref comes from: however large the scores are, the
+// largest p is 2^kBelow, or what ref's own rounding makes of it (in a fused multiply-add the product's rounding error, 64 at
+// 2^30, is left over in the argument)
 __device__ __forceinline__ float exp2_of(float v, float f, float ref) { return exp2_approx(__fsub_rn(__fmul_rn(v, f), ref)); }
 __device__ __forceinline__ bool has_nan_code(uint32_t w) {  // any byte 0x7f or 0xff
   const uint32_t m = (w & 0x7f7f7f7fu) + 0x01010101u;
@@ -801,8 +802,8 @@ __global__ void __launch_bounds__(kThreads, kNT * kD <= 256 ? 3 : 2) kv_attentio
       for (int nt = 0; nt < kNT; ++nt) {
         // a column without a token so far: any finite reference will do
         const float ref0 = m[nt][0] == kMinusInf ? 0.0f : m[nt][0], ref1 = m[nt][1] == kMinusInf ? 0.0f : m[nt][1];
-        // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Scores of 2^23 and more are a
-        // unit off in fp32, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
+        // l sums p as it was rounded: what a row's largest p is off by cancels in the quotient.  Behind scores of 2^24 and more
+        // the reference is rounded to several units, so that p may pass 2^(kBelow + kSlack) and fp16's largest.
         const auto weights = [&](auto by_share) {
 #pragma unroll
           for (int mt = 0; mt < S::kMT; ++mt) {
