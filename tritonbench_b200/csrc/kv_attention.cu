@@ -175,9 +175,11 @@ struct Shares {
   int each, rest;  // the first `rest` shares are one larger
   __device__ __forceinline__ Shares(int total, int ctas) : each(total / ctas) { rest = total - each * ctas; }
   __device__ __forceinline__ int begin(int c) const { return c * each + min(c, rest); }
-  __device__ __forceinline__ int holder(int at) const {  // CTA whose share `at` is in
+  // CTA whose share `at` is in.  Bounds that run backwards claim rows more than once: a sum of them that wraps can end inside a
+  // tile, whose end is then no CTA's.  The join must not look for its part behind the workspace.
+  __device__ __forceinline__ int holder(int at) const {
     const int large = rest * (each + 1);
-    return at < large ? at / (each + 1) : rest + (at - large) / each;
+    return min(at < large ? at / (each + 1) : rest + (at - large) / each, static_cast<int>(gridDim.x) - 1);
   }
 };
 
